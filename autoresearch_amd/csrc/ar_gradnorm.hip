@@ -1,0 +1,202 @@
+// ar_gradnorm.hip -- the norm of all gradients together, and clipping by it:
+//   norm = sqrt(sum over all tensors of g^2), out = g min(1, max_norm / norm).
+// Bound by HBM: the gradients are read once for the norm, read again to be
+// scaled and written.  Sums are fp64 in a fixed order, so that the norm is
+// right for gradients anywhere in fp32's range and the same every time.
+#include <math.h>
+
+#include <algorithm>
+#include <new>
+
+#include "ar_losses.hpp"
+
+namespace ar {
+namespace {
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+constexpr int kClipBlock = 256;
+constexpr int kClipTensors = 100;        // per launch: the table is a kernel argument
+constexpr int64_t kClipMinShare = 4096;  // elements of a block
+
+struct ClipTable {
+    const void* in[kClipTensors];
+    void* out[kClipTensors];
+    int64_t size[kClipTensors];
+    int32_t block0[kClipTensors + 1];
+    uint8_t bf16[kClipTensors];
+    int32_t n;
+};
+static_assert(sizeof(ClipTable) <= 3600, "kernel arguments hold 4 KiB");
+
+__device__ __forceinline__ int tensor_of(const ClipTable& t, int b) {
+    int lo = 0, hi = t.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (t.block0[mid] <= b) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+// Each value of block b's share of its tensor, vectors of 16 bytes where the
+// tensor starts on one.
+template <typename T, typename F>
+__device__ __forceinline__ void each(const T* in, int64_t lo, int64_t hi, F f) {
+    for (int64_t i = lo + threadIdx.x; i < hi; i += kClipBlock) f(i, to_f32<T>(in[i]));
+}
+
+__global__ __launch_bounds__(kClipBlock) void clip_sum_k(ClipTable t, int64_t share, double* part) {
+    __shared__ double red[kClipBlock / kWave];
+    const int b = blockIdx.x, j = tensor_of(t, b);
+    const int64_t lo = (b - t.block0[j]) * share, hi = min(t.size[j], lo + share);
+    double s = 0.0;
+    auto add = [&](int64_t, float v) { s = fma((double)v, (double)v, s); };
+    if (t.bf16[j]) each(static_cast<const bf16*>(t.in[j]), lo, hi, add);
+    else each(static_cast<const float*>(t.in[j]), lo, hi, add);
+    s = block_total(s, red);
+    if (threadIdx.x == 0) part[b] = s;
+}
+
+// Every block sums the np partials in the same order.  A norm that is not
+// finite clips nothing.
+__global__ __launch_bounds__(kClipBlock) void clip_scale_k(ClipTable t, int64_t share, const double* part, int64_t np,
+                                                           double max_norm, float* norm_out) {
+    __shared__ double red[kClipBlock / kWave];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < np; i += kClipBlock) s += part[i];
+    const double norm = sqrt(block_total(s, red));
+    if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = (float)norm;
+    if (t.n == 0) return;
+    const double c = norm > max_norm && norm < INFINITY ? max_norm / norm : 1.0;
+    const int b = blockIdx.x, j = tensor_of(t, b);
+    if (c == 1.0 && t.in[j] == t.out[j]) return;
+    const int64_t lo = (b - t.block0[j]) * share, hi = min(t.size[j], lo + share);
+    if (t.bf16[j]) {
+        bf16* out = static_cast<bf16*>(t.out[j]);
+        each(static_cast<const bf16*>(t.in[j]), lo, hi, [&](int64_t i, float v) { out[i] = (bf16)(float)(v * c); });
+    } else {
+        float* out = static_cast<float*>(t.out[j]);
+        each(static_cast<const float*>(t.in[j]), lo, hi, [&](int64_t i, float v) { out[i] = (float)(v * c); });
+    }
+}
+
+struct Range {
+    uintptr_t lo, hi;
+    bool written;
+};
+
+// Whether a tensor is written while another one, or part of its own input,
+// lies there too (a tensor clipped in place is one range).
+int32_t check_overlap(const char* nm, void* const* outs, const void* const* grads, const int32_t* grads_bf16,
+                      const int64_t* sizes, int64_t n) {
+    Range* r = new (std::nothrow) Range[2 * n + 1];
+    if (!r) return set_error(AR_ENOMEM, "%s: no host memory for %lld tensors", nm, (long long)n);
+    int64_t k = 0;
+    for (int64_t j = 0; j < n; ++j) {
+        const size_t bytes = (size_t)sizes[j] * (grads_bf16 && grads_bf16[j] ? 2 : 4);
+        if (!bytes) continue;
+        const uintptr_t in = reinterpret_cast<uintptr_t>(grads[j]);
+        const uintptr_t out = outs ? reinterpret_cast<uintptr_t>(outs[j]) : in;
+        r[k++] = Range{out, out + bytes, true};
+        if (out != in) r[k++] = Range{in, in + bytes, false};
+    }
+    std::sort(r, r + k, [](const Range& a, const Range& b) { return a.lo < b.lo; });
+    uintptr_t end_all = 0, end_written = 0;
+    bool bad = false;
+    for (int64_t i = 0; i < k; ++i) {
+        bad = bad || r[i].lo < (r[i].written ? end_all : end_written);
+        end_all = std::max(end_all, r[i].hi);
+        if (r[i].written) end_written = std::max(end_written, r[i].hi);
+    }
+    delete[] r;
+    AR_CHECK_ARG(!bad, "%s: tensors that are written overlap each other or the gradients", nm);
+    return AR_OK;
+}
+
+// Elements per block: about 2048 blocks for all tensors together.
+int64_t clip_share(const int64_t* sizes, int64_t n) {
+    int64_t total = 0;
+    for (int64_t j = 0; j < n; ++j) total += sizes[j];
+    return cdiv(cdiv(total, 2048) + 1, kClipMinShare) * kClipMinShare;
+}
+
+}  // namespace
+
+int64_t clip_partials(const int64_t* sizes, int64_t n) {
+    const int64_t share = clip_share(sizes, n);
+    int64_t b = 0;
+    for (int64_t j = 0; j < n; ++j) b += cdiv(sizes[j], share);
+    return b;
+}
+
+int32_t clip_grads(hipStream_t st, float* norm_out, void* const* outs, const void* const* grads,
+                   const int32_t* grads_bf16, const int64_t* sizes, int64_t n, double max_norm, double* part) {
+    const int64_t share = clip_share(sizes, n), np = clip_partials(sizes, n);
+    bool inplace = true;
+    for (int64_t j = 0; j < n; ++j) inplace = inplace && (!outs || outs[j] == grads[j] || sizes[j] == 0);
+    bool norm_done = false;
+    for (int phase = 0; phase < 2; ++phase) {
+        int64_t done = 0;
+        for (int64_t j = 0; j < n;) {
+            if (phase == 1 && inplace && !(max_norm < INFINITY)) break;  // nothing to write
+            ClipTable t;
+            t.n = 0;
+            int64_t blocks = 0;
+            for (; j < n && t.n < kClipTensors; ++j) {
+                if (sizes[j] == 0) continue;
+                t.in[t.n] = grads[j];
+                t.out[t.n] = outs ? outs[j] : const_cast<void*>(grads[j]);
+                t.size[t.n] = sizes[j];
+                t.bf16[t.n] = grads_bf16 && grads_bf16[j];
+                t.block0[t.n++] = (int32_t)blocks;
+                blocks += cdiv(sizes[j], share);
+            }
+            if (t.n == 0) break;
+            t.block0[t.n] = (int32_t)blocks;
+            if (phase == 0) {
+                clip_sum_k<<<(unsigned)blocks, kClipBlock, 0, st>>>(t, share, part + done);
+            } else {
+                clip_scale_k<<<(unsigned)blocks, kClipBlock, 0, st>>>(t, share, part, np, max_norm,
+                                                                      norm_done ? nullptr : norm_out);
+                norm_done = true;
+            }
+            done += blocks;
+        }
+    }
+    if (!norm_done) {
+        ClipTable t;
+        t.n = 0;
+        clip_scale_k<<<1, kClipBlock, 0, st>>>(t, share, part, np, max_norm, norm_out);
+    }
+    return check_launch("clip_grad_norm");
+}
+
+}  // namespace ar
+
+using namespace ar;
+
+extern "C" int32_t ar_clip_grad_norm(ar_stream_t stream, float* norm_out, void* const* outputs,
+                                     const void* const* grads, const int32_t* grads_bf16, const int64_t* sizes,
+                                     int64_t num_tensors, double max_norm) {
+    const char* nm = "clip_grad_norm";
+    AR_CHECK_ARG(norm_out && (num_tensors <= 0 || (grads && sizes)), "%s: null pointer", nm);
+    AR_CHECK_ARG(num_tensors >= 0 && num_tensors <= (1 << 24), "%s: bad number of tensors", nm);
+    AR_CHECK_ARG(max_norm > 0.0, "%s: max_norm must be positive", nm);
+    for (int64_t j = 0; j < num_tensors; ++j) {
+        const int32_t b = grads_bf16 ? grads_bf16[j] : 0;
+        AR_CHECK_ARG(b == 0 || b == 1, "%s: grads_bf16[%lld] must be 0 or 1", nm, (long long)j);
+        AR_CHECK_ARG(sizes[j] >= 0 && sizes[j] <= (int64_t(1) << 40), "%s: bad size of tensor %lld", nm, (long long)j);
+        AR_CHECK_ARG(sizes[j] == 0 || (grads[j] && (!outputs || outputs[j])), "%s: null tensor %lld", nm,
+                     (long long)j);
+        const uintptr_t mis = reinterpret_cast<uintptr_t>(grads[j]) |
+                              (outputs ? reinterpret_cast<uintptr_t>(outputs[j]) : uintptr_t(0));
+        AR_CHECK_ARG(sizes[j] == 0 || (mis & (b ? 1 : 3)) == 0, "%s: tensor %lld not aligned to a value", nm,
+                     (long long)j);
+    }
+    if (const int32_t r = check_overlap(nm, outputs, grads, grads_bf16, sizes, num_tensors)) return r;
+    int32_t status;
+    double* part = static_cast<double*>(
+        workspace(S(stream), (size_t)(clip_partials(sizes, num_tensors) + 1) * sizeof(double), &status));
+    if (!part) return status;
+    return clip_grads(S(stream), norm_out, outputs, grads, grads_bf16, sizes, num_tensors, max_norm, part);
+}

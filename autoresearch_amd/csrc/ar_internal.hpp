@@ -174,6 +174,12 @@ struct AdamTable {
 int32_t adamw_multi(hipStream_t st, float* p, const float* g, float* m, float* v, const AdamEntry* e, int n,
                     const float* sc, int bc2_i, float b2, float eps, float wd);
 
+// ---- gradient norm and clipping (ar_gradnorm.hip) ----
+// ar_clip_grad_norm on checked arguments; part: clip_partials(...) doubles.
+int64_t clip_partials(const int64_t* sizes, int64_t n);
+int32_t clip_grads(hipStream_t st, float* norm_out, void* const* outs, const void* const* grads,
+                   const int32_t* grads_bf16, const int64_t* sizes, int64_t n, double max_norm, double* part);
+
 // ---- fused row kernels of the bf16 step (ar_fused.hip) ----
 // mode 0: x0 = rmsnorm(table[idx]), x = sa[l] x0 + sb[l] x0; 1: x = sa[l] xin +
 // sb[l] x0; 2: x = xin.  Then rms, xn = bf16(x / rms); with gate_out also

@@ -1,0 +1,90 @@
+// ar_losses.hpp -- shared by the post-training losses: token log-probabilities
+// and their gradient (ar_logprob.hip), the policy and preference losses
+// (ar_losses.hip).  fp32 or bf16 logits, fp64 for the few values per token.
+#pragma once
+
+#include "ar_internal.hpp"
+
+namespace ar {
+
+// What one token adds to the policy loss, before its weight:
+//   pg = -A rho, rho = r = exp(logp - old) or the bound that binds it,
+//   kl = exp(ref - logp) - (ref - logp) - 1, loss = pg + c kl, g = d loss / d logp.
+// The bound binds where it lowers the gain: r > hi with A > 0, r < lo with
+// A < 0; there pg does not depend on logp.  In fp64: the difference of two
+// fp32 log-probabilities is exact in it, and r is compared with the bounds
+// unrounded; a few values per token cost nothing beside a row of logits.
+struct PolicyIn {
+    const float *old_logp, *ref_logp, *adv;  // old_logp null: old = logp; ref_logp null: no KL term
+    double lo, hi, kl_coef;
+};
+struct PolicyTerm {
+    double loss, kl, g;
+};
+__device__ __forceinline__ PolicyTerm policy_term(double logp, int64_t t, const PolicyIn& in) {
+    const double a = in.adv[t];
+    const double r = in.old_logp ? exp(logp - (double)in.old_logp[t]) : 1.0;
+    const bool above = a > 0.0 && r > in.hi, below = a < 0.0 && r < in.lo;
+    PolicyTerm o;
+    o.loss = -a * (above ? in.hi : below ? in.lo : r);
+    o.g = above || below ? 0.0 : -a * r;
+    o.kl = 0.0;
+    if (in.ref_logp) {
+        const double k = (double)in.ref_logp[t] - logp, e = expm1(k);
+        o.kl = e - k;
+        if (in.kl_coef != 0.0) {
+            o.loss += in.kl_coef * o.kl;
+            o.g -= in.kl_coef * e;
+        }
+    }
+    return o;
+}
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+    return v;
+}
+// As block_sum(float), for double and int; red holds blockDim.x / 64 values.
+template <typename T>
+__device__ __forceinline__ T block_total(T v, T* red) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+    const int w = threadIdx.x / kWave, l = threadIdx.x % kWave, nw = blockDim.x / kWave;
+    __syncthreads();
+    if (l == 0) red[w] = v;
+    __syncthreads();
+    T t = 0;
+    for (int i = 0; i < nw; ++i) t += red[i];
+    return t;
+}
+
+// Rows of logits (ar_logprob.hip).  FWD: logp.  BWD: the gradient by the
+// logits of sum_t grad_logp[t] logp[t].  POLICY: logp, each token's weighted
+// loss and KL to terms, and the loss's gradient by the logits; weight[t] is
+// what the token's term weighs in the loss, 0 for one that does not count.
+enum class LpOp { FWD, BWD, POLICY };
+struct LpRows {
+    const void* logits = nullptr;
+    void* grad = nullptr;  // may be logits
+    const int64_t* targets = nullptr;
+    float* logp = nullptr;
+    const float* grad_logp = nullptr;  // BWD
+    const float* weight = nullptr;     // POLICY
+    double2* terms = nullptr;          // POLICY: {loss, kl} per token
+    PolicyIn policy{};
+    float cap = 0.f;         // the softcap the logits went through, 0: none
+    float loss_scale = 1.f;  // POLICY
+    int64_t n = 0, V = 0;
+};
+int32_t lp_rows(hipStream_t st, LpOp op, bool bf16_logits, const LpRows& a, const char* nm);
+// What the entry points on logits check alike.
+int32_t check_rows(const char* nm, const void* logits, int32_t logits_bf16, const void* grad, const int64_t* targets,
+                   int64_t n, int64_t V);
+
+inline bool overlaps(const void* a, size_t na, const void* b, size_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && x < y + nb && y < x + na;
+}
+
+}  // namespace ar

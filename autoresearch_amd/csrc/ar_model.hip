@@ -31,6 +31,7 @@
 #include <vector>
 
 #include "ar_internal.hpp"
+#include "ar_losses.hpp"
 
 using namespace ar;
 
@@ -121,6 +122,8 @@ struct ar_gpt {
     size_t sort_bytes = 0;
     int32_t sort_bits = 32;
     int64_t adam_step = 0;
+    double grad_clip = 0.0;  // of train_step and train_step_graph, 0: none
+    float* grad_norm = nullptr;
     std::vector<void*> allocs;
     // profiling (ar_gpt_profile)
     bool prof = false;
@@ -335,6 +338,7 @@ static int32_t gpt_build(ar_gpt* m) {
     FALLOC(m->logits, BT * V);
     FALLOC(m->loss, BT);
     FALLOC(m->mean_loss, 64);
+    FALLOC(m->grad_norm, 64);
     FALLOC(m->dsc, 64);
     FALLOC(m->rms_final, BT);
     FALLOC(m->d_buf, BT * H);
@@ -476,6 +480,7 @@ static int32_t gpt_build(ar_gpt* m) {
     upd(BT * (C > kv ? C : kv));                  // embedding scatter partials
     upd((int64_t)kGateBlocks * H * kGateChannels);  // ve gate partials
     upd(2 * (int64_t)kNormBwdWaves);                // learned-scalar gradient partials
+    upd(2 * (clip_partials(&m->nparams, 1) + 1));   // gradient norm partials (fp64)
     m->scratch_elems = need;
     FALLOC(m->scratch, need);
     for (int i = 0; i < 2; ++i) {
@@ -682,12 +687,31 @@ static int32_t forward_bf16(ar_gpt* m, const int64_t* inputs, const int64_t* tar
     return fixed_sum(st, m->mean_loss, m->loss, nullptr, BT, 0, 0, 0, m->scratch);
 }
 
-static int32_t backward_bf16(ar_gpt* m, const int64_t* inputs, const int64_t* targets, float loss_scale) {
+// The gradient by the logits of a loss given by its gradient by the tokens'
+// log-probabilities (softcapped logits of the last forward).
+static int32_t logits_grad(ar_gpt* m, void* grad, const void* logits, bool bf16_logits, const int64_t* targets,
+                           const float* grad_logp) {
+    LpRows a;
+    a.logits = logits;
+    a.grad = grad;
+    a.targets = targets;
+    a.grad_logp = grad_logp;
+    a.cap = kSoftcap;
+    a.n = m->BT;
+    a.V = m->c.vocab_size;
+    return lp_rows(m->st, LpOp::BWD, bf16_logits, a, "gpt_backward_logp");
+}
+
+static int32_t backward_bf16(ar_gpt* m, const int64_t* inputs, const int64_t* targets, float loss_scale,
+                             const float* grad_logp = nullptr) {
     const ar_gpt_config& c = m->c;
     const int64_t C = c.n_embd, V = c.vocab_size, BT = m->BT, H = c.n_head, hd = c.head_dim, kv = c.kv_dim;
     const int64_t F = kMlpExpansion * C;
     hipStream_t st = m->st;
-    if (!m->grad_logits_valid || m->grad_logits_scale != loss_scale) {
+    if (grad_logp) {
+        AR_TRY(logits_grad(m, m->grad_logits_b, LogitsB(m), true, targets, grad_logp));
+        m->grad_logits_valid = false;
+    } else if (!m->grad_logits_valid || m->grad_logits_scale != loss_scale) {
         AR_TRY(ce_fused(st, nullptr, m->grad_logits_b, LogitsB(m), targets, BT, V, loss_scale));
         m->grad_logits_scale = loss_scale;
         m->grad_logits_valid = true;
@@ -831,12 +855,16 @@ static int32_t sort_tokens(ar_gpt* m, const int64_t* inputs) {
                              m->sort_bytes, nullptr);
 }
 
-static int32_t backward_fp32(ar_gpt* m, const int64_t* inputs, const int64_t* targets, float loss_scale) {
+static int32_t backward_fp32(ar_gpt* m, const int64_t* inputs, const int64_t* targets, float loss_scale,
+                             const float* grad_logp = nullptr) {
     const ar_gpt_config& c = m->c;
     const int64_t C = c.n_embd, V = c.vocab_size, BT = m->BT, H = c.n_head, hd = c.head_dim;
     const int64_t kv = c.kv_dim, F = kMlpExpansion * C;
     ar_stream_t st = AS(m);
-    AR_TRY(ar_cross_entropy_softcap_bwd(st, m->grad_logits, m->logits, targets, kSoftcap, BT, V, loss_scale));
+    if (grad_logp)
+        AR_TRY(logits_grad(m, m->grad_logits, m->logits, false, targets, grad_logp));
+    else
+        AR_TRY(ar_cross_entropy_softcap_bwd(st, m->grad_logits, m->logits, targets, kSoftcap, BT, V, loss_scale));
     AR_TRY(linear_dx(m, m->grad_x, m->grad_logits, P(m, m->i_lm), BT, V, C));
     AR_TRY(linear_dw(m, G(m, m->i_lm), m->grad_logits, m->x_final, BT, V, C));
     AR_TRY(ar_rmsnorm_bwd(st, m->grad_x, m->grad_x, m->x, m->rms_final, BT, C));
@@ -895,6 +923,41 @@ extern "C" int32_t ar_gpt_backward(ar_gpt* m, const int64_t* inputs, const int64
     AR_CHECK_ARG(m && inputs && targets, "gpt_backward: null pointer");
     AR_TRY(sort_tokens(m, inputs));
     return m->bf16 ? backward_bf16(m, inputs, targets, loss_scale) : backward_fp32(m, inputs, targets, loss_scale);
+}
+
+extern "C" int32_t ar_gpt_backward_logp(ar_gpt* m, const int64_t* inputs, const int64_t* targets,
+                                        const float* grad_logp) {
+    AR_CHECK_ARG(m && inputs && targets && grad_logp, "gpt_backward_logp: null pointer");
+    AR_TRY(sort_tokens(m, inputs));
+    return m->bf16 ? backward_bf16(m, inputs, targets, 0.f, grad_logp)
+                   : backward_fp32(m, inputs, targets, 0.f, grad_logp);
+}
+
+// The whole gradient arena is one tensor (its padding is zero).
+static int32_t clip_arena(ar_gpt* m, double max_norm) {
+    const void* g = m->grads;
+    return clip_grads(m->st, m->grad_norm, nullptr, &g, nullptr, &m->nparams, 1, max_norm,
+                      reinterpret_cast<double*>(m->scratch));
+}
+
+extern "C" int32_t ar_gpt_clip_grads(ar_gpt* m, double max_norm, float* norm_host) {
+    AR_CHECK_ARG(m != nullptr, "gpt_clip_grads: null model");
+    AR_CHECK_ARG(max_norm > 0.0, "gpt_clip_grads: max_norm must be positive");
+    AR_TRY(clip_arena(m, max_norm));
+    if (norm_host) {
+        if (hipMemcpyAsync(norm_host, m->grad_norm, sizeof(float), hipMemcpyDeviceToHost, m->st) != hipSuccess ||
+            hipStreamSynchronize(m->st) != hipSuccess)
+            return set_error(AR_EHIP, "gpt_clip_grads: norm copy failed");
+    }
+    return AR_OK;
+}
+
+extern "C" int32_t ar_gpt_set_grad_clip(ar_gpt* m, double max_norm) {
+    AR_CHECK_ARG(m != nullptr, "gpt_set_grad_clip: null model");
+    AR_CHECK_ARG(max_norm >= 0.0, "gpt_set_grad_clip: max_norm must not be negative");
+    if (max_norm != m->grad_clip) m->graph_in = nullptr;  // the recorded step holds the old one
+    m->grad_clip = max_norm;
+    return AR_OK;
 }
 
 // train.mojo:25-33
@@ -1073,6 +1136,7 @@ extern "C" int32_t ar_gpt_train_step(ar_gpt* m, const int64_t* inputs, const int
     AR_TRY(ar_gpt_zero_grads(m));
     AR_TRY(ar_gpt_forward(m, inputs, targets, nullptr));
     AR_TRY(ar_gpt_backward(m, inputs, targets, 1.0f));
+    if (m->grad_clip > 0.0) AR_TRY(clip_arena(m, m->grad_clip));
     AR_TRY(ar_gpt_optimizer_step(m, progress));
     if (loss_host) {
         if (hipMemcpyAsync(loss_host, m->mean_loss, sizeof(float), hipMemcpyDeviceToHost, m->st) != hipSuccess ||
@@ -1114,6 +1178,7 @@ extern "C" int32_t ar_gpt_train_step_graph(ar_gpt* m, const int64_t* inputs, con
         if (!r) r = m->bf16 ? forward_bf16(m, inputs, targets) : forward_fp32(m, inputs, targets);
         if (!r) r = sort_tokens(m, inputs);
         if (!r) r = m->bf16 ? backward_bf16(m, inputs, targets, 1.0f) : backward_fp32(m, inputs, targets, 1.0f);
+        if (!r && m->grad_clip > 0.0) r = clip_arena(m, m->grad_clip);
         if (!r) r = optimizer_kernels(m);
         const hipError_t ec = hipStreamEndCapture(m->st, &body);
         if (r) {

@@ -93,6 +93,7 @@ struct Args {
     int64_t vocab = kVocab, depth = kDepth, B = 4, T = 512;  // train.mojo:152-153
     bool fp32 = false, graph = false;
     double fake_dt = -1.0;
+    double clip = 0.0;    // --clip NORM: bound on the gradients' norm, 0: none
     int64_t nan_at = -1;  // --nan-at STEP: lm_head[0] := NaN before that step (tests the fast fail)
 };
 
@@ -119,11 +120,12 @@ Args parse(int argc, char** argv) {
         else if (k == "--seq") a.T = atoll(val());
         else if (k == "--fp32") a.fp32 = true;
         else if (k == "--graph") a.graph = true;
+        else if (k == "--clip") a.clip = atof(val());
         else if (k == "--fake-dt") a.fake_dt = atof(val());
         else if (k == "--nan-at") a.nan_at = atoll(val());
         else {
             fprintf(stderr, "usage: ar_train [--data DIR] [--tokenizer DIR] [--vocab V] [--depth D] [--batch B] "
-                            "[--seq T] [--fp32] [--graph] [--fake-dt SEC] [--nan-at STEP]\n");
+                            "[--seq T] [--fp32] [--graph] [--clip NORM] [--fake-dt SEC] [--nan-at STEP]\n");
             exit(2);
         }
     }
@@ -164,6 +166,7 @@ int main(int argc, char** argv) {
     ar_gpt* m = nullptr;
     CHECK(ar_gpt_create(&m, &cfg, B, T, a.fp32 ? AR_PREC_FP32 : AR_PREC_BF16, rope_period, ast), "gpt_create");
     CHECK(ar_gpt_init_weights(m, 42), "init_weights");  // model.mojo:347
+    CHECK(ar_gpt_set_grad_clip(m, a.clip), "grad_clip");
 
     ar_loader* train = nullptr;
     CHECK(ar_loader_create(&train, a.data.c_str(), "train", B, T, 1000), "train loader");
@@ -233,6 +236,7 @@ int main(int argc, char** argv) {
             HIPCHECK(hipMemcpyAsync(&loss32, ar_gpt_mean_loss(m), sizeof(float), hipMemcpyDeviceToHost, st), "loss");
             HIPCHECK(hipStreamSynchronize(st), "step");
             upload(cur ^ 1);
+            if (a.clip > 0.0) CHECK(ar_gpt_clip_grads(m, a.clip, nullptr), "clip_grads");
             CHECK(ar_gpt_optimizer_step(m, progress), "optimizer");
             HIPCHECK(hipStreamSynchronize(st), "optimizer");
             cur ^= 1;

@@ -123,6 +123,25 @@ class GPT:
     def backward(self, inputs, targets, loss_scale: float = 1.0):
         check(self.lib.ar_gpt_backward(self.h, _ptr(inputs), _ptr(targets), loss_scale), "gpt_backward")
 
+    def backward_logp(self, inputs, targets, grad_logp: torch.Tensor):
+        """Backward of a loss given by its gradient by the tokens' log-probabilities
+        (logp = -token_loss()), float32 [B*T]."""
+        if not (grad_logp.is_cuda and grad_logp.dtype == torch.float32 and grad_logp.is_contiguous()
+                and grad_logp.numel() == self.B * self.T):
+            raise ValueError("grad_logp must be a contiguous float32 device tensor of B*T values")
+        check(self.lib.ar_gpt_backward_logp(self.h, _ptr(inputs), _ptr(targets), grad_logp.data_ptr()),
+              "gpt_backward_logp")
+
+    def clip_grads(self, max_norm: float) -> float:
+        """Scales the gradients to a norm of at most max_norm; their norm before."""
+        norm = ct.c_float()
+        check(self.lib.ar_gpt_clip_grads(self.h, max_norm, ct.byref(norm)), "gpt_clip_grads")
+        return norm.value
+
+    def set_grad_clip(self, max_norm: float):
+        """train_step and train_step_graph clip to max_norm from now on (0: they do not)."""
+        check(self.lib.ar_gpt_set_grad_clip(self.h, max_norm), "gpt_set_grad_clip")
+
     def optimizer_step(self, progress: float = 0.0):
         check(self.lib.ar_gpt_optimizer_step(self.h, progress), "gpt_optimizer_step")
 

@@ -273,6 +273,81 @@ int32_t ar_muon_step(ar_stream_t stream, float* params, float* grads, float* mom
                      int64_t cols, double initial_lr, double lr_multiplier, double momentum,
                      double weight_decay, int32_t precision);
 
+/* ---------------- post-training (no counterpart in the reference) ----------------
+ * Token log-probabilities and their gradient, the clipped policy loss, the
+ * preference loss, and the gradient norm with clipping.
+ *
+ * Logits are fp32 (logits_bf16 0) or bf16 (1) [num_tokens, vocab_size],
+ * contiguous, of any size and alignment to a value, as ar_softcap_fwd or
+ * ar_lm_head_softcap_ce_bf16 leave them; `cap` is the softcap they went through
+ * (z = cap tanh(x / cap)), 0 for none, and gradients are by x: unlike
+ * ar_cross_entropy_softcap_bwd they carry the factor 1 - (z / cap)^2.
+ *
+ * A token counts if 0 <= target < vocab_size and, where there are sequences,
+ * it lies in one: sequence s holds tokens seq_start[s] .. seq_start[s + 1] - 1
+ * (device, num_seqs + 1 ascending offsets in [0, num_tokens]; offsets beyond it
+ * or descending ones shorten sequences).  A token that does not count has
+ * log-probability 0 and gradient 0, whatever its logits or other inputs hold:
+ * they are not read.  Sums over tokens are fp64, in a fixed order.
+ *
+ * num_tokens up to 2^31 - 1, vocab_size up to 2^30 (AR_EUNSUPPORTED above).
+ * Arrays of no elements may be NULL. */
+
+/* logp_out[t] = z[t, targets[t]] - log sum_j exp(z[t, j]) */
+int32_t ar_token_logprob_fwd(ar_stream_t stream, float* logp_out, const void* logits, int32_t logits_bf16,
+                             const int64_t* targets, int64_t num_tokens, int64_t vocab_size);
+/* grad_logits[t, j] = grad_logp[t] ([j = targets[t]] - softmax(z[t])[j]) (1 - (z[t, j] / cap)^2),
+ * of the logits' type; may alias logits.  A token with grad_logp 0 does not count. */
+int32_t ar_token_logprob_bwd(ar_stream_t stream, void* grad_logits, const void* logits, int32_t logits_bf16,
+                             const int64_t* targets, const float* grad_logp, float cap, int64_t num_tokens,
+                             int64_t vocab_size);
+/* The clipped policy loss with a KL term, and its gradient by logp:
+ *   r = exp(logp - old_logp), k = ref_logp - logp, A = advantages[t],
+ *   L_t = max(-A r, -A min(max(r, 1 - clip_low), 1 + clip_high)) + kl_coef (e^k - k - 1),
+ *   loss_out[0] = sum_t w_t L_t, loss_out[1] = sum_t w_t (e^k - k - 1),
+ *   grad_logp[t] = loss_scale d loss_out[0] / d logp[t]
+ * with w_t = 1 / (tokens that count), or with per_seq
+ * 1 / (sequences with a token that counts x the sequence's tokens that count).
+ * Without a token that counts all outputs are 0.  old_logp NULL: old_logp =
+ * logp, held fixed (r = 1).  ref_logp NULL: no KL term (kl_coef 0, loss_out[1]
+ * 0).  grad_logp NULL: the loss alone; it may alias logp.  seq_start NULL: the
+ * tokens are one sequence (num_seqs 1).  Takes scratch from the workspace. */
+int32_t ar_policy_loss(ar_stream_t stream, float* loss_out, float* grad_logp, const float* logp,
+                       const float* old_logp, const float* ref_logp, const float* advantages, const int64_t* targets,
+                       const int64_t* seq_start, double clip_low, double clip_high, double kl_coef, int32_t per_seq,
+                       int64_t num_tokens, int64_t num_seqs, int64_t vocab_size, float loss_scale);
+/* The same from the logits, with its gradient by them, in one pass over the
+ * logits: ar_token_logprob_fwd, ar_policy_loss and ar_token_logprob_bwd.
+ * grad_logits may alias logits; logp_out may be NULL. */
+int32_t ar_policy_loss_logits(ar_stream_t stream, float* loss_out, float* logp_out, void* grad_logits,
+                              const void* logits, int32_t logits_bf16, const float* old_logp, const float* ref_logp,
+                              const float* advantages, const int64_t* targets, const int64_t* seq_start, float cap,
+                              double clip_low, double clip_high, double kl_coef, int32_t per_seq, int64_t num_tokens,
+                              int64_t num_seqs, int64_t vocab_size, float loss_scale);
+/* The preference loss over pairs of sequences (2 i chosen, 2 i + 1 rejected):
+ *   h_i = beta (sum over the chosen's tokens that count of (logp - ref_logp) - the same of the rejected's),
+ *   loss_out[0] = mean_i of -(1 - label_smoothing) log sigma(h_i) - label_smoothing log sigma(-h_i),
+ *   margin_out[i] = h_i, grad_logp[t] = loss_scale d loss_out[0] / d logp[t].
+ * A pair with a sequence in which no token counts is left out of the mean
+ * (margin and gradients 0).  ref_logp NULL: 0.  grad_logp and margin_out may be
+ * NULL; grad_logp must not overlap logp or ref_logp.  seq_start: 2 num_pairs + 1
+ * offsets.  Takes scratch from the workspace. */
+int32_t ar_preference_loss(ar_stream_t stream, float* loss_out, float* margin_out, float* grad_logp,
+                           const float* logp, const float* ref_logp, const int64_t* targets, const int64_t* seq_start,
+                           double beta, double label_smoothing, int64_t num_tokens, int64_t num_pairs,
+                           int64_t vocab_size, float loss_scale);
+/* norm_out[0] = the 2-norm of all gradients together; outputs[i] = grads[i]
+ * min(1, max_norm / norm).  grads, outputs, grads_bf16 and sizes are host
+ * arrays of num_tensors device pointers, types (1 = bf16, 0 = fp32; NULL: all
+ * fp32) and element counts; they are read before the call returns.  outputs
+ * NULL, or outputs[i] == grads[i]: in place, and gradients within max_norm are
+ * not touched.  A tensor that is written must overlap no other.  max_norm
+ * INFINITY: the norm alone.  A norm that is not finite is returned as it is and
+ * clips nothing (outputs = grads): the caller drops the step.  The norm is
+ * summed in fp64 in a fixed order.  Takes scratch from the workspace. */
+int32_t ar_clip_grad_norm(ar_stream_t stream, float* norm_out, void* const* outputs, const void* const* grads,
+                          const int32_t* grads_bf16, const int64_t* sizes, int64_t num_tensors, double max_norm);
+
 /* ---------------- model.mojo init ---------------- */
 
 /* model.mojo:86-115  xorshift + Box-Muller N(0, std) */
@@ -332,6 +407,21 @@ int32_t ar_gpt_zero_grads(ar_gpt* model);
 int32_t ar_gpt_forward(ar_gpt* model, const int64_t* inputs, const int64_t* targets, float* loss_host);
 /* model.mojo:819-1037 (quirks of the reference backward reproduced) */
 int32_t ar_gpt_backward(ar_gpt* model, const int64_t* inputs, const int64_t* targets, float loss_scale);
+/* The backward of any loss on the tokens' log-probabilities (logp[t] =
+ * -token_loss[t]), given by its gradient grad_logp (device, [B*T]) by them: what
+ * ar_policy_loss and ar_preference_loss return.  No counterpart in the
+ * reference.  The gradient by the logits carries the softcap's derivative, which
+ * ar_gpt_backward leaves out as the reference does; everything behind them is
+ * ar_gpt_backward's. */
+int32_t ar_gpt_backward_logp(ar_gpt* model, const int64_t* inputs, const int64_t* targets, const float* grad_logp);
+/* Between backward and optimizer step: scales all gradients by min(1, max_norm
+ * / their norm) (ar_clip_grad_norm on the arena; max_norm INFINITY: the norm
+ * alone).  If norm_host is non-NULL the call synchronises and stores the norm
+ * there.  No counterpart in the reference. */
+int32_t ar_gpt_clip_grads(ar_gpt* model, double max_norm, float* norm_host);
+/* ar_gpt_train_step and ar_gpt_train_step_graph clip to max_norm from now on
+ * (0, as created: they do not clip).  A graph is recorded anew. */
+int32_t ar_gpt_set_grad_clip(ar_gpt* model, double max_norm);
 /* train.mojo:246-281: AdamW groups then Muon on all 2-D matrices */
 int32_t ar_gpt_optimizer_step(ar_gpt* model, double progress);
 /* train.mojo:231-282: zero_grads -> forward -> backward(1.0) -> optimizer */
