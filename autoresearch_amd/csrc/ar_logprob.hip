@@ -102,31 +102,59 @@ __device__ __forceinline__ MaxSum block_max_sum(MaxSum v, float* red) {
     return t;
 }
 
-// What a token's gradient by its log-probability is, and for POLICY its terms;
-// by one thread of a workgroup.
+// A token's values for POLICY, loaded ahead of its row; nothing otherwise.
 template <LpOp OP>
-__device__ __forceinline__ float row_coef(const LpRows& a, int64_t r, float w, float logp) {
-    if constexpr (OP == LpOp::POLICY) {
-        const PolicyTerm t = policy_term(logp, r, a.policy);
+struct RowToken {
+    __device__ __forceinline__ RowToken(const LpRows&, int64_t) {}
+    // The gradient by logp; w: the token's weight or gradient.
+    __device__ __forceinline__ float coef(const LpRows&, int64_t, float w, float) const { return w; }
+};
+template <>
+struct RowToken<LpOp::POLICY> {
+    PolicyToken t;
+    __device__ __forceinline__ RowToken(const LpRows& a, int64_t r) : t(a.policy, r) {}
+    __device__ __forceinline__ float coef(const LpRows& a, int64_t r, float w, float logp) const {
+        const PolicyTerm<float> o = policy_term<float>(logp, t, a.policy);
         if (a.logp) a.logp[r] = logp;
-        a.terms[r] = make_double2(w * t.loss, w * t.kl);
-        return (float)(w * t.g * a.loss_scale);
+        a.terms[r] = make_double2((double)w * o.loss, (double)w * o.kl);
+        return w * o.g * a.loss_scale;
     }
-    return w;
-}
+};
+
+// exp(z - m).  SUB: the difference first.  Otherwise one fma and the hardware's
+// exponential: z log2 e - m log2 e, rounded once.  The second product's own
+// rounding is a factor common to the whole row, which the sum has too; it is
+// small up to |m| = 2^20, and the caller sees to that.
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+constexpr float kFar = 1048576.f;
+template <bool SUB>
+struct RowExp {
+    float m, c;
+    __device__ __forceinline__ explicit RowExp(float max) : m(max), c(max * -kLog2e) {}
+    __device__ __forceinline__ float log2_of(float z) const {
+        return SUB ? (z - m) * kLog2e : fmaf(z, kLog2e, c);
+    }
+    __device__ __forceinline__ float operator()(float z) const { return __builtin_amdgcn_exp2f(log2_of(z)); }
+    // log-probability of z where the row's exponentials sum up to s
+    __device__ __forceinline__ float logp(float z, float s) const { return (log2_of(z) - log2f(s)) * kLn2; }
+};
 
 // The gradient of a value that is not the target: -g p f; the target's has
-// g f besides, f = 1 - (z / cap)^2.
+// g f besides, f = 1 - (z / cap)^2 (values past the cap by rounding: 0).
+// z0: what the values were shortened by.
+template <bool SUB>
 struct RowGrad {
-    float m, gs, rcap;  // gs = g / sum
-    __device__ __forceinline__ RowGrad(const LpRows& a, float g, MaxSum v)
-        : m(v.m), gs(-g / v.s), rcap(a.cap > 0.f ? 1.f / a.cap : 0.f) {}
+    RowExp<SUB> ex;
+    float g, sum, gs, rcap, u0;  // gs = -g / sum
+    __device__ __forceinline__ RowGrad(RowExp<SUB> e, float cap, float coef, float s, float z0)
+        : ex(e), g(coef), sum(s), gs(-coef / s), rcap(cap > 0.f ? 1.f / cap : 0.f), u0(z0 * rcap) {}
     __device__ __forceinline__ float factor(float z) const {
-        const float u = z * rcap;
-        return fmaxf(0.f, fmaf(-u, u, 1.f));
+        const float u = fmaf(z, rcap, u0);
+        return fminf(fmaxf(fmaf(-u, u, 1.f), 0.f), 1.f);
     }
-    __device__ __forceinline__ float operator()(float z) const { return gs * __expf(z - m) * factor(z); }
-    __device__ __forceinline__ float target(float z, float g) const { return fmaf(gs, __expf(z - m), g) * factor(z); }
+    __device__ __forceinline__ float operator()(float z) const { return gs * ex(z) * factor(z); }
+    // (a target that holds the whole row: exactly 0)
+    __device__ __forceinline__ float target(float z) const { return g * (1.f - ex(z) / sum) * factor(z); }
 };
 
 template <typename T>
@@ -152,69 +180,34 @@ __device__ __forceinline__ bool row_counts(const LpRows& a, int64_t r, int64_t y
     return false;
 }
 
-// The maximum and sum of 16 bytes of a row.
-template <typename T>
-__device__ __forceinline__ void add_chunk(MaxSum& v, u32x4 q) {
+// The maximum and sum of N chunks of a row, the sum so far rescaled once.
+template <typename T, int N>
+__device__ __forceinline__ void add_chunks(MaxSum& v, const u32x4* q) {
     using R = Row<T>;
-    float cm = R::get(q, 0);
+    float cm = R::get(q[0], 0);
 #pragma unroll
-    for (int i = 1; i < R::E; ++i) cm = fmaxf(cm, R::get(q, i));
-    const float use = fmaxf(v.m, cm) == -INFINITY ? 0.f : fmaxf(v.m, cm);
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int i = 0; i < R::E; ++i) cm = fmaxf(cm, R::get(q[k], i));
+    const float nm = fmaxf(v.m, cm), use = nm == -INFINITY ? 0.f : nm;
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < R::E; ++i) s += __expf(R::get(q, i) - use);
-    v.add(cm == -INFINITY ? -INFINITY : use, s);
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int i = 0; i < R::E; ++i) s += __expf(R::get(q[k], i) - use);
+    v.s = fmaf(v.s, __expf(v.m - use), s);
+    v.m = nm;
 }
 
 // Between two passes over held chunks: what the first one made of them (bf16
 // values widened to fp32: twice the registers) is made again, not kept.
 __device__ __forceinline__ void again(u32x4& q) { asm volatile("" : "+v"(q)); }
 
-constexpr int kRowBlock = 256;
+constexpr int kBatch = 4;  // chunks a lane has in flight
 
 // Rows of any length: the row is read again for the gradient.
-template <typename T, LpOp OP>
-__global__ __launch_bounds__(kRowBlock) void lp_row_k(LpRows a) {
-    using R = Row<T>;
-    constexpr int E = R::E;
-    __shared__ float red[2 * kRowBlock / kWave];
-    __shared__ float coef;
-    const int64_t r = blockIdx.x;
-    const int V = (int)a.V, tid = threadIdx.x;
-    const int64_t y = a.targets[r];
-    const T* row = static_cast<const T*>(a.logits) + r * a.V;
-    T* out = static_cast<T*>(a.grad) + r * a.V;
-    float w;
-    if (!row_counts<T, OP>(a, r, y, w)) return;
-    const Span<T> sp(row, V);
-    const int h = sp.h, nb = sp.nb, ej = sp.edge(tid, V);
-    const float zy = to_f32<T>(row[y]), ez = ej >= 0 ? to_f32<T>(row[ej]) : -INFINITY;
-    MaxSum v;
-    for (int c = tid; c < nb; c += kRowBlock) add_chunk<T>(v, R::load(row + h + c * E));
-    v.add(ez, ez == -INFINITY ? 0.f : __expf(ez - ez));
-    v = block_max_sum(v, red);
-    if constexpr (OP == LpOp::FWD) {
-        if (tid == 0) a.logp[r] = (zy - v.m) - logf(v.s);
-        return;
-    }
-    if (tid == 0) coef = row_coef<OP>(a, r, w, (zy - v.m) - logf(v.s));
-    __syncthreads();  // zy and the sums are read: from here the row may be overwritten
-    const float g = coef;
-    const RowGrad grad(a, g, v);
-    for (int c = tid; c < nb; c += kRowBlock) {
-        const u32x4 q = R::load(row + h + c * E);
-        float x[E];
-#pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = h + c * E + i == y ? grad.target(zy, g) : grad(R::get(q, i));
-        R::store(out + h + c * E, R::pack(x));
-    }
-    if (ej >= 0) out[ej] = from_f32<T>(ej == y ? grad.target(zy, g) : grad(ez));
-}
-
-// The same for rows of up to NV TB chunks of 16 bytes, held in registers: one
-// read, and the maximum before the exponentials.
-template <typename T, LpOp OP, int TB, int NV>
-__global__ __launch_bounds__(TB, NV > 8 ? 4 : 6) void lp_held_k(LpRows a) {
+template <typename T, LpOp OP, int TB>
+__global__ __launch_bounds__(TB) void lp_row_k(LpRows a) {
     using R = Row<T>;
     constexpr int E = R::E;
     __shared__ float red[2 * (TB / kWave)];
@@ -226,80 +219,165 @@ __global__ __launch_bounds__(TB, NV > 8 ? 4 : 6) void lp_held_k(LpRows a) {
     T* out = static_cast<T*>(a.grad) + r * a.V;
     float w;
     if (!row_counts<T, OP>(a, r, y, w)) return;
+    const RowToken<OP> token(a, r);
+    const Span<T> sp(row, V);
+    const int h = sp.h, nb = sp.nb, ej = sp.edge(tid, V);
+    const float zy = to_f32<T>(row[y]), ez = ej >= 0 ? to_f32<T>(row[ej]) : -INFINITY;
+    const int whole = nb / (kBatch * TB) * (kBatch * TB);  // chunks in batches that every lane fills
+    MaxSum v;
+    u32x4 q[kBatch];
+    for (int c = tid; c < whole; c += kBatch * TB) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) q[k] = R::load(row + h + (c + k * TB) * E);
+        add_chunks<T, kBatch>(v, q);
+    }
+    for (int c = whole + tid; c < nb; c += TB) {
+        q[0] = R::load(row + h + c * E);
+        add_chunks<T, 1>(v, q);
+    }
+    v.add(ez, ez == -INFINITY ? 0.f : __expf(ez - ez));
+    v = block_max_sum(v, red);
+    if constexpr (OP == LpOp::FWD) {
+        if (tid == 0) a.logp[r] = (zy - v.m) - logf(v.s);
+        return;
+    }
+    if (tid == 0) coef = token.coef(a, r, w, (zy - v.m) - logf(v.s));
+    __syncthreads();  // zy and the sums are read: from here the row may be overwritten
+    const RowGrad<true> grad(RowExp<true>(v.m), a.cap, coef, v.s, 0.f);
+    auto emit = [&](int c, u32x4 z) {
+        float x[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = h + c * E + i == y ? grad.target(zy) : grad(R::get(z, i));
+        R::store(out + h + c * E, R::pack(x));
+    };
+    for (int c = tid; c < whole; c += kBatch * TB) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) q[k] = R::load(row + h + (c + k * TB) * E);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) emit(c + k * TB, q[k]);
+    }
+    for (int c = whole + tid; c < nb; c += TB) emit(c, R::load(row + h + c * E));
+    if (ej >= 0) out[ej] = from_f32<T>(ej == y ? grad.target(zy) : grad(ez));
+}
+
+// The same for rows of up to NV TB chunks of 16 bytes, held in registers: one
+// read, and the maximum before the exponentials.  Only rows with a chunk may
+// come to an instance with SURE > 0: its first SURE steps ask no question (the
+// row's last chunk is loaded where a lane has none, and not used).
+template <typename T, LpOp OP, int TB, int NV, int SURE>
+__global__ __launch_bounds__(TB, NV > 8 ? 4 : 8) void lp_held_k(LpRows a) {
+    using R = Row<T>;
+    constexpr int E = R::E;
+    __shared__ float red[2 * (TB / kWave)];
+    __shared__ float coef;
+    const int64_t r = blockIdx.x;
+    const int V = (int)a.V, tid = threadIdx.x;
+    const int64_t y = a.targets[r];
+    const T* row = static_cast<const T*>(a.logits) + r * a.V;
+    T* out = static_cast<T*>(a.grad) + r * a.V;
+    float w;
+    if (!row_counts<T, OP>(a, r, y, w)) return;
+    const RowToken<OP> token(a, r);
     const Span<T> sp(row, V);
     const int h = sp.h, nb = sp.nb;
     const u32x4 none = R::fill(-INFINITY);
     u32x4 q[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k)
-        if (k * TB < nb) {
+        if (k < SURE || k * TB < nb) {
             const int c = tid + k * TB;
             q[k] = R::load(row + h + min(c, nb - 1) * E);
         }
     const int ej = sp.edge(tid, V);
-    const float ez = ej >= 0 ? to_f32<T>(row[ej]) : -INFINITY;
-    const float zy = to_f32<T>(row[y]);
+    float ez = ej >= 0 ? to_f32<T>(row[ej]) : -INFINITY;
+    float zy = to_f32<T>(row[y]);
     float mt = ez;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
-        if (k * TB < nb) {
+        if (k < SURE || k * TB < nb) {
             if (tid + k * TB >= nb) q[k] = none;
 #pragma unroll
             for (int i = 0; i < E; ++i) mt = fmaxf(mt, R::get(q[k], i));
             again(q[k]);
         }
-    MaxSum v;
-    v.m = block_max(mt, red);
-    const float use = v.m == -INFINITY ? 0.f : v.m;
-    float st = __expf(ez - use);
+    float m = block_max(mt, red);
+    float z0 = 0.f;
+    if (__builtin_amdgcn_readfirstlane(!(fabsf(m) < kFar))) {
+        // the same in every lane: shorten the row by its maximum.  (Values
+        // that bf16 rounds here differ from it by 2^12 or more: no weight.)
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            float x[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] = R::get(q[k], i) - m;
+            q[k] = R::pack(x);
+            again(q[k]);
+        }
+        ez -= m;
+        zy -= m;
+        z0 = m;
+        m = 0.f;
+    }
+    const RowExp<false> ex(m);
+    float st = ex(ez);
 #pragma unroll
     for (int k = 0; k < NV; ++k)
-        if (k * TB < nb) {
+        if (k < SURE || k * TB < nb) {
             float s = 0.f;
 #pragma unroll
-            for (int i = 0; i < E; ++i) s += __expf(R::get(q[k], i) - use);
+            for (int i = 0; i < E; ++i) s += ex(R::get(q[k], i));
             st += s;
             again(q[k]);
         }
-    v.s = block_sum(st, red + TB / kWave);
-    if (tid == 0) coef = row_coef<OP>(a, r, w, (zy - v.m) - logf(v.s));
+    st = block_sum(st, red + TB / kWave);
+    if (tid == 0) coef = token.coef(a, r, w, ex.logp(zy, st));
     __syncthreads();
-    const float g = coef;
-    const RowGrad grad(a, g, v);
+    const RowGrad<false> grad(ex, a.cap, coef, st, z0);
     const int yc = y < h ? -1 : ((int)y - h) / E, yi = y < h ? 0 : ((int)y - h) % E;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
-        if (k * TB < nb) {
+        if (k < SURE || k * TB < nb) {
             const int c = tid + k * TB;
             float x[E];
 #pragma unroll
             for (int i = 0; i < E; ++i) x[i] = grad(R::get(q[k], i));
             if (c == yc) {
-                const float t = grad.target(zy, g);
+                const float t = grad.target(zy);
 #pragma unroll
                 for (int i = 0; i < E; ++i) x[i] = i == yi ? t : x[i];
             }
             if (c < nb) R::store(out + h + c * E, R::pack(x));
         }
-    if (ej >= 0) out[ej] = from_f32<T>(ej == y ? grad.target(zy, g) : grad(ez));
+    if (ej >= 0) out[ej] = from_f32<T>(ej == y ? grad.target(zy) : grad(ez));
 }
 
+// Lanes and chunks per lane by the row's chunks.  Measured (fp32, TB/s of the
+// row read and the gradient written): with as few chunks per lane as 1024 lanes
+// allow, down to two, a row is in flight the shortest: 8192 values 1024 x 2 6.1,
+// 512 x 4 5.4, 256 x 8 5.5; 16384 values 1024 x 4 6.0, 512 x 8 5.3.  bf16 has
+// twice the values per chunk and takes four: 8192 values 256 x 4 5.8, 512 x 2
+// 5.6, 1024 x 1 3.7.
 template <typename T, LpOp OP>
 void launch_grad(hipStream_t st, const LpRows& a) {
     const unsigned g = (unsigned)a.n;
     const int64_t nc = cdiv(a.V, Row<T>::E);
-    if (nc <= 128) lp_held_k<T, OP, 64, 2><<<g, 64, 0, st>>>(a);
-    else if (nc <= 512) lp_held_k<T, OP, 64, 8><<<g, 64, 0, st>>>(a);
-    else if (nc <= 2048) lp_held_k<T, OP, 256, 8><<<g, 256, 0, st>>>(a);
-    else if (nc <= 4096) lp_held_k<T, OP, 256, 16><<<g, 256, 0, st>>>(a);
-    else if (nc <= 8192) lp_held_k<T, OP, 512, 16><<<g, 512, 0, st>>>(a);
-    else if (nc <= 16384) lp_held_k<T, OP, 1024, 16><<<g, 1024, 0, st>>>(a);
-    else lp_row_k<T, OP><<<g, kRowBlock, 0, st>>>(a);
+#define AR_HELD(TB, NV) lp_held_k<T, OP, TB, NV, NV / 2><<<g, TB, 0, st>>>(a)
+    constexpr int M = sizeof(T) == 2 ? 4 : 2;
+    if (nc <= 64 * 2) lp_held_k<T, OP, 64, 2, 0><<<g, 64, 0, st>>>(a);  // rows without a whole chunk too
+    else if (nc <= 128 * M) AR_HELD(128, M);
+    else if (nc <= 256 * M) AR_HELD(256, M);
+    else if (nc <= 512 * M) AR_HELD(512, M);
+    else if (nc <= 1024 * M) AR_HELD(1024, M);
+    else if (nc <= 1024 * 4) AR_HELD(1024, 4);
+    else if (nc <= 1024 * 8) AR_HELD(1024, 8);
+    else if (nc <= 1024 * 16) AR_HELD(1024, 16);
+    else lp_row_k<T, OP, 1024><<<g, 1024, 0, st>>>(a);
+#undef AR_HELD
 }
 
 template <typename T>
 int32_t launch(hipStream_t st, LpOp op, const LpRows& a, const char* nm) {
-    if (op == LpOp::FWD) lp_row_k<T, LpOp::FWD><<<(unsigned)a.n, kRowBlock, 0, st>>>(a);
+    if (op == LpOp::FWD) lp_row_k<T, LpOp::FWD, 256><<<(unsigned)a.n, 256, 0, st>>>(a);
     else if (op == LpOp::BWD) launch_grad<T, LpOp::BWD>(st, a);
     else launch_grad<T, LpOp::POLICY>(st, a);
     return check_launch(nm);

@@ -102,7 +102,7 @@ __global__ __launch_bounds__(kTokBlock) void policy_tokens_k(const float* weight
         const float w = weight[t];
         float g = 0.f;
         if (w != 0.f) {
-            const PolicyTerm o = policy_term(logp[t], t, in);
+            const PolicyTerm<double> o = policy_term<double>(logp[t], PolicyToken(in, t), in);
             loss += w * o.loss;
             kl += w * o.kl;
             g = (float)(w * o.g * loss_scale);

@@ -11,30 +11,41 @@ namespace ar {
 //   pg = -A rho, rho = r = exp(logp - old) or the bound that binds it,
 //   kl = exp(ref - logp) - (ref - logp) - 1, loss = pg + c kl, g = d loss / d logp.
 // The bound binds where it lowers the gain: r > hi with A > 0, r < lo with
-// A < 0; there pg does not depend on logp.  In fp64: the difference of two
-// fp32 log-probabilities is exact in it, and r is compared with the bounds
-// unrounded; a few values per token cost nothing beside a row of logits.
+// A < 0; there pg does not depend on logp.
+// F = double where log-probabilities are given: the difference of two fp32
+// values is exact in it, and r meets the bounds unrounded.  F = float where
+// they come out of a row of logits: what fp32 adds to their own error (a few
+// 1e-7) is less, and one lane's fp64 exponentials held up the row (65536 rows
+// of 8192 fp32 values: 798 us, in fp32 and with the token's values loaded
+// ahead 725).
 struct PolicyIn {
     const float *old_logp, *ref_logp, *adv;  // old_logp null: old = logp; ref_logp null: no KL term
     double lo, hi, kl_coef;
 };
-struct PolicyTerm {
-    double loss, kl, g;
+struct PolicyToken {
+    float adv, old_logp, ref_logp;
+    __device__ __forceinline__ PolicyToken(const PolicyIn& in, int64_t t)
+        : adv(in.adv[t]), old_logp(in.old_logp ? in.old_logp[t] : 0.f), ref_logp(in.ref_logp ? in.ref_logp[t] : 0.f) {}
 };
-__device__ __forceinline__ PolicyTerm policy_term(double logp, int64_t t, const PolicyIn& in) {
-    const double a = in.adv[t];
-    const double r = in.old_logp ? exp(logp - (double)in.old_logp[t]) : 1.0;
-    const bool above = a > 0.0 && r > in.hi, below = a < 0.0 && r < in.lo;
-    PolicyTerm o;
-    o.loss = -a * (above ? in.hi : below ? in.lo : r);
-    o.g = above || below ? 0.0 : -a * r;
-    o.kl = 0.0;
+template <typename F>
+struct PolicyTerm {
+    F loss, kl, g;
+};
+template <typename F>
+__device__ __forceinline__ PolicyTerm<F> policy_term(F logp, const PolicyToken& t, const PolicyIn& in) {
+    const F a = t.adv, lo = (F)in.lo, hi = (F)in.hi, c = (F)in.kl_coef;
+    const F r = in.old_logp ? exp(logp - (F)t.old_logp) : (F)1;
+    const bool above = a > (F)0 && r > hi, below = a < (F)0 && r < lo;
+    PolicyTerm<F> o;
+    o.loss = -a * (above ? hi : below ? lo : r);
+    o.g = above || below ? (F)0 : -a * r;
+    o.kl = (F)0;
     if (in.ref_logp) {
-        const double k = (double)in.ref_logp[t] - logp, e = expm1(k);
+        const F k = (F)t.ref_logp - logp, e = expm1(k);
         o.kl = e - k;
-        if (in.kl_coef != 0.0) {
-            o.loss += in.kl_coef * o.kl;
-            o.g -= in.kl_coef * e;
+        if (c != (F)0) {
+            o.loss += c * o.kl;
+            o.g -= c * e;
         }
     }
     return o;

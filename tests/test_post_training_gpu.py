@@ -165,6 +165,34 @@ def test_rows_of_infinities_and_nan(env, V, dtype, n):
     close(torch, out[live], d, tol, dt)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("V", [9, 513, 8192, 40001, 150001, 270001])
+def test_rows_of_far_values(env, V, dtype):
+    """Rows whose largest value is far from zero, on both sides of 2^20, or the type's lowest or largest value."""
+    torch, ops = env
+    dt = getattr(torch, dtype)
+    top = [1048575.0, 1048576.0, 1.0e6, 3.0e6, -1.0e6, -3.0e6, 1e9, -1e9, 3e37, torch.finfo(dt).min, torch.finfo(dt).max]
+    n = len(top)
+    g = gen(torch, V)
+    z = (torch.tensor(top, device="cuda", dtype=torch.float64)[:, None]
+         - torch.rand(n, V, generator=g, device="cuda").double() * 4).clamp(torch.finfo(dt).min, torch.finfo(dt).max).to(dt)
+    z[:, 0] = torch.tensor(top, device="cuda", dtype=torch.float64).to(dt)
+    y = torch.randint(0, V, (n,), generator=g, device="cuda")
+    z[2, 1:] = 0.0  # one value holds all
+    z[3, V // 2:] = -math.inf
+    y[3] = 0
+    gl = torch.ones(n, device="cuda")
+    logp, out = torch.empty(n, device="cuda"), torch.empty_like(z)
+    ops.token_logprob_fwd(logp, z, y, n, V)
+    ops.token_logprob_bwd(out, z, y, gl, 0.0, n, V)
+    want, p, lse, m, z_y, ok = ref_rows(torch, z, y)
+    want = (z_y - m) - torch.log(torch.exp(z.double() - m[:, None]).sum(1))  # lse itself is rounded to the values' size
+    close(torch, logp, want, logp_tol(V, z_y, m, m + torch.log(torch.exp(z.double() - m[:, None]).sum(1)), want)
+          + U * 4 * math.log(V), torch.float32)
+    d, tol = ref_grad(torch, z, y, p, ok, gl, 0.0)
+    close(torch, out, d, tol, dt)
+
+
 # ---------------------------------------------------------------- policy
 
 def ref_weights(torch, y, start, V, per_seq):
