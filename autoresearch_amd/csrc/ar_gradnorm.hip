@@ -13,7 +13,6 @@
 namespace ar {
 namespace {
 
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kClipBlock = 256;
 constexpr int kClipTensors = 100;        // per launch: the table is a kernel argument
 constexpr int64_t kClipMinShare = 4096;  // elements of a block
@@ -38,21 +37,57 @@ __device__ __forceinline__ int tensor_of(const ClipTable& t, int b) {
     return lo;
 }
 
-// Each value of block b's share of its tensor, vectors of 16 bytes where the
-// tensor starts on one.
-template <typename T, typename F>
-__device__ __forceinline__ void each(const T* in, int64_t lo, int64_t hi, F f) {
-    for (int64_t i = lo + threadIdx.x; i < hi; i += kClipBlock) f(i, to_f32<T>(in[i]));
+constexpr int kClipBatch = 4;  // loads of 16 bytes that a lane has in flight
+
+// f(chunk's first element, chunk) for every whole chunk of in[lo .. hi), and
+// g(element, value) for the values behind the last one.
+template <typename T, typename F, typename G>
+__device__ __forceinline__ void each(const void* base, int64_t lo, int64_t hi, F f, G g) {
+    using R = Row<T>;
+    constexpr int64_t E = R::E, step = kClipBlock * E;
+    const T* in = static_cast<const T*>(base);
+    int64_t i = lo + threadIdx.x * E;
+    for (; i + (kClipBatch - 1) * step + E <= hi; i += kClipBatch * step) {
+        u32x4 q[kClipBatch];
+#pragma unroll
+        for (int k = 0; k < kClipBatch; ++k) q[k] = R::load(in + i + k * step);
+#pragma unroll
+        for (int k = 0; k < kClipBatch; ++k) f(i + k * step, q[k]);
+    }
+    for (; i + E <= hi; i += step) f(i, R::load(in + i));
+    for (int64_t j = hi - (hi - lo) % E + threadIdx.x; j < hi; j += kClipBlock) g(j, to_f32<T>(in[j]));
+}
+
+template <typename T>
+__device__ __forceinline__ double sum_squares(const void* in, int64_t lo, int64_t hi) {
+    double s = 0.0;
+    auto add = [&](float v) { s = fma((double)v, (double)v, s); };
+    each<T>(in, lo, hi,
+            [&](int64_t, u32x4 q) {
+#pragma unroll
+                for (int e = 0; e < Row<T>::E; ++e) add(Row<T>::get(q, e));
+            },
+            [&](int64_t, float v) { add(v); });
+    return s;
+}
+template <typename T>
+__device__ __forceinline__ void scale(const void* in, void* out, int64_t lo, int64_t hi, double c) {
+    T* o = static_cast<T*>(out);
+    each<T>(in, lo, hi,
+            [&](int64_t i, u32x4 q) {
+                float x[Row<T>::E];
+#pragma unroll
+                for (int e = 0; e < Row<T>::E; ++e) x[e] = (float)(Row<T>::get(q, e) * c);
+                Row<T>::store(o + i, Row<T>::pack(x));
+            },
+            [&](int64_t i, float v) { o[i] = from_f32<T>((float)(v * c)); });
 }
 
 __global__ __launch_bounds__(kClipBlock) void clip_sum_k(ClipTable t, int64_t share, double* part) {
     __shared__ double red[kClipBlock / kWave];
     const int b = blockIdx.x, j = tensor_of(t, b);
     const int64_t lo = (b - t.block0[j]) * share, hi = min(t.size[j], lo + share);
-    double s = 0.0;
-    auto add = [&](int64_t, float v) { s = fma((double)v, (double)v, s); };
-    if (t.bf16[j]) each(static_cast<const bf16*>(t.in[j]), lo, hi, add);
-    else each(static_cast<const float*>(t.in[j]), lo, hi, add);
+    double s = t.bf16[j] ? sum_squares<bf16>(t.in[j], lo, hi) : sum_squares<float>(t.in[j], lo, hi);
     s = block_total(s, red);
     if (threadIdx.x == 0) part[b] = s;
 }
@@ -68,16 +103,12 @@ __global__ __launch_bounds__(kClipBlock) void clip_scale_k(ClipTable t, int64_t 
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = (float)norm;
     if (t.n == 0) return;
     const double c = norm > max_norm && norm < INFINITY ? max_norm / norm : 1.0;
-    const int b = blockIdx.x, j = tensor_of(t, b);
+    // back to front: what the sums read last is the likeliest still cached
+    const int b = gridDim.x - 1 - blockIdx.x, j = tensor_of(t, b);
     if (c == 1.0 && t.in[j] == t.out[j]) return;
     const int64_t lo = (b - t.block0[j]) * share, hi = min(t.size[j], lo + share);
-    if (t.bf16[j]) {
-        bf16* out = static_cast<bf16*>(t.out[j]);
-        each(static_cast<const bf16*>(t.in[j]), lo, hi, [&](int64_t i, float v) { out[i] = (bf16)(float)(v * c); });
-    } else {
-        float* out = static_cast<float*>(t.out[j]);
-        each(static_cast<const float*>(t.in[j]), lo, hi, [&](int64_t i, float v) { out[i] = (float)(v * c); });
-    }
+    if (t.bf16[j]) scale<bf16>(t.in[j], t.out[j], lo, hi, c);
+    else scale<float>(t.in[j], t.out[j], lo, hi, c);
 }
 
 struct Range {

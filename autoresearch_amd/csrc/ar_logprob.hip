@@ -14,45 +14,6 @@
 namespace ar {
 namespace {
 
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-
-// 16 bytes of a row: E values.  Rows start at any multiple of a value's size
-// (any V, any view), which the vector accesses say.
-template <typename T>
-struct Row;
-template <>
-struct Row<float> {
-    static constexpr int E = 4;
-    typedef u32x4 vec __attribute__((aligned(4)));
-    static __device__ __forceinline__ float get(u32x4 v, int i) { return __uint_as_float(v[i]); }
-    static __device__ __forceinline__ u32x4 pack(const float* x) {
-        u32x4 v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(x[i]);
-        return v;
-    }
-    static __device__ __forceinline__ u32x4 load(const float* p) { return *reinterpret_cast<const vec*>(p); }
-    static __device__ __forceinline__ void store(float* p, u32x4 v) { *reinterpret_cast<vec*>(p) = v; }
-    static __device__ __forceinline__ u32x4 fill(float x) { return u32x4{1, 1, 1, 1} * __float_as_uint(x); }
-};
-template <>
-struct Row<bf16> {
-    static constexpr int E = 8;
-    typedef u32x4 vec __attribute__((aligned(2)));
-    static __device__ __forceinline__ float get(u32x4 v, int i) {
-        return __uint_as_float((i & 1) ? (v[i / 2] & 0xffff0000u) : (v[i / 2] << 16));
-    }
-    static __device__ __forceinline__ u32x4 pack(const float* x) {
-        bf16x8 b;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) b[i] = (bf16)x[i];
-        return __builtin_bit_cast(u32x4, b);
-    }
-    static __device__ __forceinline__ u32x4 load(const bf16* p) { return *reinterpret_cast<const vec*>(p); }
-    static __device__ __forceinline__ void store(bf16* p, u32x4 v) { *reinterpret_cast<vec*>(p) = v; }
-    static __device__ __forceinline__ u32x4 fill(float x) { return u32x4{1, 1, 1, 1} * (__float_as_uint(x) >> 16) * 0x10001u; }
-};
-
 // A row's values in chunks of 16 bytes: h values before them, V - tail0 < E
 // behind them.  Accesses of 16 bytes cost the same at any multiple of 4 bytes
 // (rows of 50001 fp32 values: 169 us either way), but more at odd multiples of

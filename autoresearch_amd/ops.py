@@ -10,6 +10,8 @@ bfloat16.  Nothing here computes on the host.
 """
 from __future__ import annotations
 
+from array import array
+
 import torch
 
 from ._lib import check, load
@@ -29,7 +31,9 @@ __all__ = [
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    # torch.cuda.current_stream().cuda_stream without the stream object around
+    # it, which takes 3 us to make: as long as a small call's kernel
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 class Workspace:
@@ -273,106 +277,115 @@ def precompute_rope(cos_buf, sin_buf, seq_len, head_dim, base=10000.0):
 _LOGITS = (torch.float32, torch.bfloat16)
 
 
-def _dev(name: str, t, n: int, dtypes=(torch.float32,), optional: bool = False):
-    """The address of a device array of at least n elements of one of dtypes."""
-    if t is None:
-        if optional or n == 0:
-            return None
-        raise ValueError(f"{name}: device tensor required")
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name}: tensor on {t.device}, not on the current device")
-    if t.dtype not in dtypes:
-        raise TypeError(f"{name}: unsupported dtype {t.dtype}")
+def _device(nm: str, t) -> int:
+    """The device of a call's first tensor: the current one."""
+    d = -1 if t is None else t.get_device()
+    if d < 0 or d != torch.cuda.current_device():
+        raise ValueError(f"{nm}: tensors on the current device are required")
+    return d
+
+
+def _dev(nm: str, what: str, t, n: int, dev: int, dtype=torch.float32, optional: bool = False):
+    """The address of an array of at least n elements of dtype on device dev."""
+    if t is None and (optional or n == 0):
+        return None
+    if t is None or t.get_device() != dev:
+        raise ValueError(f"{nm} {what}: a tensor on the current device is required")
+    if t.dtype is not dtype:
+        raise TypeError(f"{nm} {what}: unsupported dtype {t.dtype}")
     if not t.is_contiguous():
-        raise ValueError(f"{name}: tensor must be contiguous")
+        raise ValueError(f"{nm} {what}: tensor must be contiguous")
     if t.numel() < n:
-        raise ValueError(f"{name}: {t.numel()} elements, {n} needed")
+        raise ValueError(f"{nm} {what}: {t.numel()} elements, {n} needed")
     return t.data_ptr()
 
 
-def _rows(name: str, logits, num_tokens, vocab_size, grad=None):
-    p = _dev(name + " logits", logits, num_tokens * vocab_size, _LOGITS)
-    bf16 = int(logits is not None and logits.dtype == torch.bfloat16)
-    if grad is None:
-        return p, bf16, None
-    if logits is not None and grad.dtype != logits.dtype:
-        raise TypeError(f"{name} grad_logits: {grad.dtype}, logits are {logits.dtype}")
-    return p, bf16, _dev(name + " grad_logits", grad, num_tokens * vocab_size, _LOGITS)
+def _logits(nm: str, logits, grad, num_tokens, vocab_size, dev):
+    """Addresses of the logits and their gradient, and whether they are bf16."""
+    dtype = torch.float32 if logits is None else logits.dtype
+    if dtype not in _LOGITS:
+        raise TypeError(f"{nm} logits: unsupported dtype {dtype}")
+    n = num_tokens * vocab_size
+    return (_dev(nm, "logits", logits, n, dev, dtype),
+            None if grad is None else _dev(nm, "grad_logits", grad, n, dev, dtype), int(dtype is torch.bfloat16))
 
 
-def _launch(name: str, *args):
-    check(getattr(load(), "ar_" + name)(_stream(), *args), name)
+def _launch(nm: str, *args):
+    check(getattr(load(), "ar_" + nm)(_stream(), *args), nm)
 
 
 def token_logprob_fwd(logp_out, logits, targets, num_tokens, vocab_size):
     """logp_out[t] = logits[t, targets[t]] - logsumexp(logits[t]); 0 where the target is no token."""
-    nm = "token_logprob_fwd"
-    p, bf16, _ = _rows(nm, logits, num_tokens, vocab_size)
-    _launch(nm, _dev(nm + " logp_out", logp_out, num_tokens), p, bf16,
-            _dev(nm + " targets", targets, num_tokens, (torch.int64,)), num_tokens, vocab_size)
+    nm, n, dev = "token_logprob_fwd", num_tokens, _device("token_logprob_fwd", logp_out)
+    z, _, bf16 = _logits(nm, logits, None, n, vocab_size, dev)
+    _launch(nm, _dev(nm, "logp_out", logp_out, n, dev), z, bf16, _dev(nm, "targets", targets, n, dev, torch.int64), n,
+            vocab_size)
 
 
 def token_logprob_bwd(grad_logits, logits, targets, grad_logp, cap, num_tokens, vocab_size):
     """The gradient of sum_t grad_logp[t] logp[t] by the logits before the softcap `cap` (0: none)."""
-    nm = "token_logprob_bwd"
-    p, bf16, g = _rows(nm, logits, num_tokens, vocab_size, grad_logits)
-    _launch(nm, g, p, bf16, _dev(nm + " targets", targets, num_tokens, (torch.int64,)),
-            _dev(nm + " grad_logp", grad_logp, num_tokens), cap, num_tokens, vocab_size)
+    nm, n, dev = "token_logprob_bwd", num_tokens, _device("token_logprob_bwd", grad_logits)
+    z, g, bf16 = _logits(nm, logits, grad_logits, n, vocab_size, dev)
+    _launch(nm, g, z, bf16, _dev(nm, "targets", targets, n, dev, torch.int64),
+            _dev(nm, "grad_logp", grad_logp, n, dev), cap, n, vocab_size)
 
 
-def _batch(nm, old_logp, ref_logp, advantages, targets, seq_start, num_tokens, num_seqs):
-    n, ids = num_tokens, (torch.int64,)
-    return (_dev(nm + " old_logp", old_logp, n, optional=True), _dev(nm + " ref_logp", ref_logp, n, optional=True),
-            _dev(nm + " advantages", advantages, n), _dev(nm + " targets", targets, n, ids),
-            _dev(nm + " seq_start", seq_start, num_seqs + 1, ids, optional=True))
+def _batch(nm, old_logp, ref_logp, advantages, targets, seq_start, n, num_seqs, dev):
+    return (_dev(nm, "old_logp", old_logp, n, dev, optional=True),
+            _dev(nm, "ref_logp", ref_logp, n, dev, optional=True), _dev(nm, "advantages", advantages, n, dev),
+            _dev(nm, "targets", targets, n, dev, torch.int64),
+            _dev(nm, "seq_start", seq_start, num_seqs + 1, dev, torch.int64, optional=True))
 
 
 def policy_loss(loss_out, grad_logp, logp, old_logp, ref_logp, advantages, targets, seq_start, clip_low, clip_high,
                 kl_coef, per_seq, num_tokens, num_seqs, vocab_size, loss_scale=1.0):
     """loss_out = (clipped policy loss with its KL term, mean KL); grad_logp = its gradient (None: not formed)."""
-    nm = "policy_loss"
-    _launch(nm, _dev(nm + " loss_out", loss_out, 2), _dev(nm + " grad_logp", grad_logp, num_tokens, optional=True),
-            _dev(nm + " logp", logp, num_tokens),
-            *_batch(nm, old_logp, ref_logp, advantages, targets, seq_start, num_tokens, num_seqs), clip_low, clip_high,
-            kl_coef, int(per_seq), num_tokens, num_seqs, vocab_size, loss_scale)
+    nm, n, dev = "policy_loss", num_tokens, _device("policy_loss", loss_out)
+    _launch(nm, _dev(nm, "loss_out", loss_out, 2, dev), _dev(nm, "grad_logp", grad_logp, n, dev, optional=True),
+            _dev(nm, "logp", logp, n, dev),
+            *_batch(nm, old_logp, ref_logp, advantages, targets, seq_start, n, num_seqs, dev), clip_low, clip_high,
+            kl_coef, int(per_seq), n, num_seqs, vocab_size, loss_scale)
 
 
 def policy_loss_logits(loss_out, logp_out, grad_logits, logits, old_logp, ref_logp, advantages, targets, seq_start,
                        cap, clip_low, clip_high, kl_coef, per_seq, num_tokens, num_seqs, vocab_size, loss_scale=1.0):
     """policy_loss from the logits, with its gradient by them (before the softcap), in one pass over them."""
-    nm = "policy_loss_logits"
-    if grad_logits is None:
-        raise ValueError(f"{nm} grad_logits: device tensor required")
-    p, bf16, g = _rows(nm, logits, num_tokens, vocab_size, grad_logits)
-    _launch(nm, _dev(nm + " loss_out", loss_out, 2), _dev(nm + " logp_out", logp_out, num_tokens, optional=True), g, p,
-            bf16, *_batch(nm, old_logp, ref_logp, advantages, targets, seq_start, num_tokens, num_seqs), cap, clip_low,
-            clip_high, kl_coef, int(per_seq), num_tokens, num_seqs, vocab_size, loss_scale)
+    nm, n, dev = "policy_loss_logits", num_tokens, _device("policy_loss_logits", loss_out)
+    z, g, bf16 = _logits(nm, logits, grad_logits, n, vocab_size, dev)
+    _launch(nm, _dev(nm, "loss_out", loss_out, 2, dev), _dev(nm, "logp_out", logp_out, n, dev, optional=True), g, z,
+            bf16, *_batch(nm, old_logp, ref_logp, advantages, targets, seq_start, n, num_seqs, dev), cap, clip_low,
+            clip_high, kl_coef, int(per_seq), n, num_seqs, vocab_size, loss_scale)
 
 
 def preference_loss(loss_out, margin_out, grad_logp, logp, ref_logp, targets, seq_start, beta, label_smoothing,
                     num_tokens, num_pairs, vocab_size, loss_scale=1.0):
     """The preference loss of pairs of sequences (2 i chosen, 2 i + 1 rejected), their margins and the gradient."""
-    nm, n = "preference_loss", num_tokens
-    _launch(nm, _dev(nm + " loss_out", loss_out, 1), _dev(nm + " margin_out", margin_out, num_pairs, optional=True),
-            _dev(nm + " grad_logp", grad_logp, n, optional=True), _dev(nm + " logp", logp, n),
-            _dev(nm + " ref_logp", ref_logp, n, optional=True), _dev(nm + " targets", targets, n, (torch.int64,)),
-            _dev(nm + " seq_start", seq_start, 2 * num_pairs + 1, (torch.int64,)), beta, label_smoothing, n, num_pairs,
+    nm, n, dev = "preference_loss", num_tokens, _device("preference_loss", loss_out)
+    _launch(nm, _dev(nm, "loss_out", loss_out, 1, dev),
+            _dev(nm, "margin_out", margin_out, num_pairs, dev, optional=True),
+            _dev(nm, "grad_logp", grad_logp, n, dev, optional=True), _dev(nm, "logp", logp, n, dev),
+            _dev(nm, "ref_logp", ref_logp, n, dev, optional=True),
+            _dev(nm, "targets", targets, n, dev, torch.int64),
+            _dev(nm, "seq_start", seq_start, 2 * num_pairs + 1, dev, torch.int64), beta, label_smoothing, n, num_pairs,
             vocab_size, loss_scale)
 
 
 def clip_grad_norm(norm_out, outputs, grads, max_norm):
     """norm_out = the 2-norm of all of grads; outputs[i] = grads[i] min(1, max_norm / norm).
     outputs None: in place.  max_norm math.inf: the norm alone."""
-    import ctypes as ct
-    nm, n = "clip_grad_norm", len(grads)
-    if outputs is not None and len(outputs) != n:
-        raise ValueError(f"{nm}: {len(outputs)} outputs for {n} gradients")
-    pg, po = (ct.c_void_p * n)(), (ct.c_void_p * n)() if outputs is not None else None
-    bf16, sizes = (ct.c_int32 * n)(), (ct.c_int64 * n)()
-    for i, g in enumerate(grads):
-        sizes[i] = g.numel()
-        pg[i] = _dev(nm + " grads", g, 0, _LOGITS)
-        bf16[i] = g.dtype == torch.bfloat16
-        if po is not None:
-            po[i] = _dev(nm + " outputs", outputs[i], sizes[i], (g.dtype,))
-    _launch(nm, _dev(nm + " norm_out", norm_out, 1), po, pg, bf16, sizes, n, max_norm)
+    if outputs is not None and len(outputs) != len(grads):
+        raise ValueError(f"clip_grad_norm: {len(outputs)} outputs for {len(grads)} gradients")
+    nm, n, dev = "clip_grad_norm", len(grads), _device("clip_grad_norm", norm_out)
+    types, sizes = [g.dtype for g in grads], [g.numel() for g in grads]
+    for t in set(types).difference(_LOGITS):
+        raise TypeError(f"{nm} grads: unsupported dtype {t}")
+
+    def addresses(what, tensors):
+        return array("Q", [_dev(nm, what, t, k, dev, d) for t, k, d in zip(tensors, sizes, types)])
+
+    def at(a):
+        return None if a is None else a.buffer_info()[0]
+
+    pg, po = addresses("grads", grads), None if outputs is None else addresses("outputs", outputs)
+    bf16, sz = array("i", [t is torch.bfloat16 for t in types]), array("q", sizes)
+    _launch(nm, _dev(nm, "norm_out", norm_out, 1, dev), at(po), at(pg), at(bf16), at(sz), n, max_norm)

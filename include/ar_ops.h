@@ -285,8 +285,8 @@ int32_t ar_muon_step(ar_stream_t stream, float* params, float* grads, float* mom
  *
  * A token counts if 0 <= target < vocab_size and, where there are sequences,
  * it lies in one: sequence s holds tokens seq_start[s] .. seq_start[s + 1] - 1
- * (device, num_seqs + 1 ascending offsets in [0, num_tokens]; offsets beyond it
- * or descending ones shorten sequences).  A token that does not count has
+ * (device, num_seqs + 1 ascending offsets in [0, num_tokens]; with others, which
+ * tokens count is not defined, but nothing outside the arrays is touched).  A token that does not count has
  * log-probability 0 and gradient 0, whatever its logits or other inputs hold:
  * they are not read.  Sums over tokens are fp64, in a fixed order.
  *
@@ -310,15 +310,16 @@ int32_t ar_token_logprob_bwd(ar_stream_t stream, void* grad_logits, const void* 
  * 1 / (sequences with a token that counts x the sequence's tokens that count).
  * Without a token that counts all outputs are 0.  old_logp NULL: old_logp =
  * logp, held fixed (r = 1).  ref_logp NULL: no KL term (kl_coef 0, loss_out[1]
- * 0).  grad_logp NULL: the loss alone; it may alias logp.  seq_start NULL: the
- * tokens are one sequence (num_seqs 1).  Takes scratch from the workspace. */
+ * 0).  grad_logp NULL: the loss alone; it may be logp or another input, not
+ * overlap one in part.  seq_start NULL: the
+ * tokens are one sequence (num_seqs 1).  May take scratch from the workspace. */
 int32_t ar_policy_loss(ar_stream_t stream, float* loss_out, float* grad_logp, const float* logp,
                        const float* old_logp, const float* ref_logp, const float* advantages, const int64_t* targets,
                        const int64_t* seq_start, double clip_low, double clip_high, double kl_coef, int32_t per_seq,
                        int64_t num_tokens, int64_t num_seqs, int64_t vocab_size, float loss_scale);
 /* The same from the logits, with its gradient by them, in one pass over the
  * logits: ar_token_logprob_fwd, ar_policy_loss and ar_token_logprob_bwd.
- * grad_logits may alias logits; logp_out may be NULL. */
+ * grad_logits may be logits; logp_out may be NULL. */
 int32_t ar_policy_loss_logits(ar_stream_t stream, float* loss_out, float* logp_out, void* grad_logits,
                               const void* logits, int32_t logits_bf16, const float* old_logp, const float* ref_logp,
                               const float* advantages, const int64_t* targets, const int64_t* seq_start, float cap,
@@ -331,7 +332,7 @@ int32_t ar_policy_loss_logits(ar_stream_t stream, float* loss_out, float* logp_o
  * A pair with a sequence in which no token counts is left out of the mean
  * (margin and gradients 0).  ref_logp NULL: 0.  grad_logp and margin_out may be
  * NULL; grad_logp must not overlap logp or ref_logp.  seq_start: 2 num_pairs + 1
- * offsets.  Takes scratch from the workspace. */
+ * offsets.  May take scratch from the workspace. */
 int32_t ar_preference_loss(ar_stream_t stream, float* loss_out, float* margin_out, float* grad_logp,
                            const float* logp, const float* ref_logp, const int64_t* targets, const int64_t* seq_start,
                            double beta, double label_smoothing, int64_t num_tokens, int64_t num_pairs,
@@ -344,7 +345,7 @@ int32_t ar_preference_loss(ar_stream_t stream, float* loss_out, float* margin_ou
  * not touched.  A tensor that is written must overlap no other.  max_norm
  * INFINITY: the norm alone.  A norm that is not finite is returned as it is and
  * clips nothing (outputs = grads): the caller drops the step.  The norm is
- * summed in fp64 in a fixed order.  Takes scratch from the workspace. */
+ * summed in fp64 in a fixed order.  May take scratch from the workspace. */
 int32_t ar_clip_grad_norm(ar_stream_t stream, float* norm_out, void* const* outputs, const void* const* grads,
                           const int32_t* grads_bf16, const int64_t* sizes, int64_t num_tensors, double max_norm);
 

@@ -111,6 +111,7 @@ def test_losses(lib, call, kw, word):
 @pytest.mark.parametrize("kw,word", [
     ({"adv": None}, "null"), ({"lo": -0.1}, "clip"), ({"hi": math.nan}, "clip"), ({"ref": None}, "ref_logp"),
     ({"kl": math.nan}, "KL"), ({"S": -1}, "shape"), ({"start": None, "S": 3}, "seq_start"),
+    ({"old": A["grad"] + 4, "ref": A["logp"] + 4}, "overlaps"), ({"adv": A["logp"] - 8, "grad": A["logp"]}, "overlaps"),
 ])
 def test_policy(lib, call, kw, word):
     refused(lib, call(lib, **kw), EINVAL, word)

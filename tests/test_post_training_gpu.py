@@ -581,8 +581,13 @@ def test_refusals(env):
     with torch.cuda.stream(side):  # no workspace is bound to it
         with pytest.raises(ArError, match="workspace"):
             ops.clip_grad_norm(f[:1], None, [f[8:]], 1.0)
+        many, ids = torch.zeros(9000, device="cuda"), torch.zeros(9000, dtype=torch.int64, device="cuda")
         with pytest.raises(ArError, match="workspace"):
-            ops.policy_loss(f, None, f, None, None, f, i, None, 0.2, 0.2, 0.0, False, 8, 1, 8)
+            ops.policy_loss(f, None, many, None, None, many, ids, None, 0.2, 0.2, 0.0, False, 9000, 1, 8)
+        with pytest.raises(ArError, match="workspace"):
+            ops.preference_loss(f, None, None, many, None, ids, ids, 0.1, 0.0, 9000, 100, 8)
+        with pytest.raises(ArError, match="workspace"):
+            ops.policy_loss_logits(f, None, many, many, None, None, f, i, None, 0.0, 0.2, 0.2, 0.0, False, 8, 1, 8)
 
 
 def test_two_streams_with_their_own_workspaces(env):
