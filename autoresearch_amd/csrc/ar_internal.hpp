@@ -175,8 +175,8 @@ int32_t adamw_multi(hipStream_t st, float* p, const float* g, float* m, float* v
                     const float* sc, int bc2_i, float b2, float eps, float wd);
 
 // ---- gradient norm and clipping (ar_gradnorm.hip) ----
-// ar_clip_grad_norm on checked arguments; part: clip_partials(...) doubles.
-int64_t clip_partials(const int64_t* sizes, int64_t n);
+// ar_clip_grad_norm on checked arguments; part: clip_partials(n) doubles.
+int64_t clip_partials(int64_t n);
 int32_t clip_grads(hipStream_t st, float* norm_out, void* const* outs, const void* const* grads,
                    const int32_t* grads_bf16, const int64_t* sizes, int64_t n, double max_norm, double* part);
 

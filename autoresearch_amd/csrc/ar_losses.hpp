@@ -26,6 +26,9 @@ struct Row<float> {
     }
     static __device__ __forceinline__ u32x4 load(const float* p) { return *reinterpret_cast<const vec*>(p); }
     static __device__ __forceinline__ void store(float* p, u32x4 v) { *reinterpret_cast<vec*>(p) = v; }
+    static __device__ __forceinline__ void store_nt(float* p, u32x4 v) {
+        __builtin_nontemporal_store(v, reinterpret_cast<vec*>(p));
+    }
     static __device__ __forceinline__ u32x4 fill(float x) { return u32x4{1, 1, 1, 1} * __float_as_uint(x); }
 };
 template <>
@@ -43,6 +46,9 @@ struct Row<bf16> {
     }
     static __device__ __forceinline__ u32x4 load(const bf16* p) { return *reinterpret_cast<const vec*>(p); }
     static __device__ __forceinline__ void store(bf16* p, u32x4 v) { *reinterpret_cast<vec*>(p) = v; }
+    static __device__ __forceinline__ void store_nt(bf16* p, u32x4 v) {
+        __builtin_nontemporal_store(v, reinterpret_cast<vec*>(p));
+    }
     static __device__ __forceinline__ u32x4 fill(float x) { return u32x4{1, 1, 1, 1} * (__float_as_uint(x) >> 16) * 0x10001u; }
 };
 

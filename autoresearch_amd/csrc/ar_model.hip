@@ -480,7 +480,7 @@ static int32_t gpt_build(ar_gpt* m) {
     upd(BT * (C > kv ? C : kv));                  // embedding scatter partials
     upd((int64_t)kGateBlocks * H * kGateChannels);  // ve gate partials
     upd(2 * (int64_t)kNormBwdWaves);                // learned-scalar gradient partials
-    upd(2 * (clip_partials(&m->nparams, 1) + 1));   // gradient norm partials (fp64)
+    upd(2 * clip_partials(1));                      // gradient norm partials (fp64)
     m->scratch_elems = need;
     FALLOC(m->scratch, need);
     for (int i = 0; i < 2; ++i) {
