@@ -193,7 +193,8 @@ int32_t clip_grads(hipStream_t st, float* norm_out, void* const* outs, const voi
                    const int32_t* grads_bf16, const int64_t* sizes, int64_t n, double max_norm, double* part) {
     const int64_t share = clip_share(grads_bf16, sizes, n);
     bool write = false;  // whether there is anything to write: a bound, or an output elsewhere
-    for (int64_t j = 0; j < n; ++j) write = write || (sizes[j] && (max_norm < INFINITY || (outs && outs[j] != grads[j])));
+    for (int64_t j = 0; j < n; ++j)
+        write = write || (sizes[j] && (max_norm < INFINITY || (outs && outs[j] != grads[j])));
     ClipTable t;
     int64_t np = 0;
     for (int64_t j = 0; j < n;)

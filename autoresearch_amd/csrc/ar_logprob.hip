@@ -67,17 +67,17 @@ __device__ __forceinline__ MaxSum block_max_sum(MaxSum v, float* red) {
 template <LpOp OP>
 struct RowToken {
     __device__ __forceinline__ RowToken(const LpRows&, int64_t) {}
-    // The gradient by logp; w: the token's weight or gradient.
-    __device__ __forceinline__ float coef(const LpRows&, int64_t, float w, float) const { return w; }
+    // The gradient by logp; w: the token's weight or gradient; out: write what else the token has.
+    __device__ __forceinline__ float coef(const LpRows&, int64_t, float w, float, bool) const { return w; }
 };
 template <>
 struct RowToken<LpOp::POLICY> {
     PolicyToken t;
     __device__ __forceinline__ RowToken(const LpRows& a, int64_t r) : t(a.policy, r) {}
-    __device__ __forceinline__ float coef(const LpRows& a, int64_t r, float w, float logp) const {
+    __device__ __forceinline__ float coef(const LpRows& a, int64_t r, float w, float logp, bool out) const {
         const PolicyTerm<float> o = policy_term<float>(logp, t, a.policy);
-        if (a.logp) a.logp[r] = logp;
-        a.terms[r] = make_double2((double)w * o.loss, (double)w * o.kl);
+        if (out && a.logp) a.logp[r] = logp;
+        if (out) a.terms[r] = make_double2((double)w * o.loss, (double)w * o.kl);
         return w * o.g * a.loss_scale;
     }
 };
@@ -126,17 +126,23 @@ __device__ __forceinline__ void zero_row(T* out, int V) {
     for (int j = nb * R::E + threadIdx.x; j < V; j += blockDim.x) out[j] = from_f32<T>(0.f);
 }
 
-// Whether a token's logits are read; if not, its outputs are written here.
-template <typename T, LpOp OP>
-__device__ __forceinline__ bool row_counts(const LpRows& a, int64_t r, int64_t y, float& w) {
+// Whether a token's logits are read; if not, its outputs but for the row are
+// written here (out).
+template <LpOp OP>
+__device__ __forceinline__ bool row_live(const LpRows& a, int64_t r, int64_t y, float& w, bool out) {
     w = 1.f;
     if constexpr (OP == LpOp::BWD) w = a.grad_logp[r];
     if constexpr (OP == LpOp::POLICY) w = a.weight[r];
     if (y >= 0 && y < a.V && w != 0.f) return true;
     if constexpr (OP != LpOp::BWD)
-        if (threadIdx.x == 0 && a.logp) a.logp[r] = 0.f;
+        if (out && threadIdx.x == 0 && a.logp) a.logp[r] = 0.f;
     if constexpr (OP == LpOp::POLICY)
-        if (threadIdx.x == 0) a.terms[r] = make_double2(0.0, 0.0);
+        if (out && threadIdx.x == 0) a.terms[r] = make_double2(0.0, 0.0);
+    return false;
+}
+template <typename T, LpOp OP>
+__device__ __forceinline__ bool row_counts(const LpRows& a, int64_t r, int64_t y, float& w) {
+    if (row_live<OP>(a, r, y, w, true)) return true;
     if constexpr (OP != LpOp::FWD) zero_row(static_cast<T*>(a.grad) + r * a.V, (int)a.V);
     return false;
 }
@@ -202,7 +208,7 @@ __global__ __launch_bounds__(TB) void lp_row_k(LpRows a) {
         if (tid == 0) a.logp[r] = (zy - v.m) - logf(v.s);
         return;
     }
-    if (tid == 0) coef = token.coef(a, r, w, (zy - v.m) - logf(v.s));
+    if (tid == 0) coef = token.coef(a, r, w, (zy - v.m) - logf(v.s), true);
     __syncthreads();  // zy and the sums are read: from here the row may be overwritten
     const RowGrad<true> grad(RowExp<true>(v.m), a.cap, coef, v.s, 0.f);
     auto emit = [&](int c, u32x4 z) {
@@ -291,7 +297,7 @@ __global__ __launch_bounds__(TB, NV > 8 ? 4 : 8) void lp_held_k(LpRows a) {
             again(q[k]);
         }
     st = block_sum(st, red + TB / kWave);
-    if (tid == 0) coef = token.coef(a, r, w, ex.logp(zy, st));
+    if (tid == 0) coef = token.coef(a, r, w, ex.logp(zy, st), true);
     __syncthreads();
     const RowGrad<false> grad(ex, a.cap, coef, st, z0);
     const int yc = y < h ? -1 : ((int)y - h) / E, yi = y < h ? 0 : ((int)y - h) % E;
@@ -310,6 +316,118 @@ __global__ __launch_bounds__(TB, NV > 8 ? 4 : 8) void lp_held_k(LpRows a) {
             if (c < nb) R::store(out + h + c * E, R::pack(x));
         }
     if (ej >= 0) out[ej] = from_f32<T>(ej == y ? grad.target(zy) : grad(ez));
+}
+
+// ---- few long rows: each split over several workgroups ----
+// part[r][p]: the maximum and sum of part p's chunks, part 0 with the values
+// outside the chunks; zy[r]: the target's.
+struct Split {
+    MaxSum* part;
+    float* zy;
+    int parts;
+    __device__ __forceinline__ int lo(int nb) const { return min(nb, (int)blockIdx.x * ((nb + parts - 1) / parts)); }
+    __device__ __forceinline__ int hi(int nb) const { return min(nb, lo(nb) + (nb + parts - 1) / parts); }
+};
+constexpr int kSplitBlock = 256;
+
+template <typename T, LpOp OP>
+__global__ __launch_bounds__(kSplitBlock) void lp_part_k(LpRows a, Split sp) {
+    using R = Row<T>;
+    __shared__ float red[2 * (kSplitBlock / kWave)];
+    const int64_t r = blockIdx.y;
+    const int V = (int)a.V, tid = threadIdx.x;
+    const int64_t y = a.targets[r];
+    float w;
+    if (!row_live<OP>(a, r, y, w, false)) return;
+    const T* row = static_cast<const T*>(a.logits) + r * a.V;
+    const Span<T> s(row, V);
+    const int hi = sp.hi(s.nb), ej = blockIdx.x == 0 ? s.edge(tid, V) : -1;
+    MaxSum v;
+    u32x4 q[kBatch];
+    int c = sp.lo(s.nb) + tid;
+    for (; c + (kBatch - 1) * kSplitBlock < hi; c += kBatch * kSplitBlock) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) q[k] = R::load(row + s.h + (c + k * kSplitBlock) * R::E);
+        add_chunks<T, kBatch>(v, q);
+    }
+    for (; c < hi; c += kSplitBlock) {
+        q[0] = R::load(row + s.h + c * R::E);
+        add_chunks<T, 1>(v, q);
+    }
+    if (ej >= 0) {
+        const float ez = to_f32<T>(row[ej]);
+        v.add(ez, ez == -INFINITY ? 0.f : __expf(ez - ez));
+    }
+    v = block_max_sum(v, red);
+    if (tid == 0) {
+        sp.part[r * sp.parts + blockIdx.x] = v;
+        if (blockIdx.x == 0) sp.zy[r] = to_f32<T>(row[y]);
+    }
+}
+// The whole row's, by every wave.
+__device__ __forceinline__ MaxSum join_parts(const Split& sp, int64_t r) {
+    const int lane = threadIdx.x % kWave;
+    MaxSum v;
+    if (lane < sp.parts) v = sp.part[r * sp.parts + lane];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const float om = __shfl_xor(v.m, o, kWave), os = __shfl_xor(v.s, o, kWave);
+        v.add(om, os);
+    }
+    return v;
+}
+__global__ __launch_bounds__(kWave) void lp_join_k(LpRows a, Split sp) {
+    const int64_t r = blockIdx.x;
+    float w;
+    if (!row_live<LpOp::FWD>(a, r, a.targets[r], w, true)) return;
+    const MaxSum v = join_parts(sp, r);
+    if (threadIdx.x == 0) a.logp[r] = (sp.zy[r] - v.m) - logf(v.s);
+}
+template <typename T, LpOp OP>
+__global__ __launch_bounds__(kSplitBlock) void lp_apply_k(LpRows a, Split sp) {
+    using R = Row<T>;
+    constexpr int E = R::E;
+    __shared__ float coef;
+    const int64_t r = blockIdx.y;
+    const int V = (int)a.V, tid = threadIdx.x;
+    const int64_t y = a.targets[r];
+    const T* row = static_cast<const T*>(a.logits) + r * a.V;
+    T* out = static_cast<T*>(a.grad) + r * a.V;
+    const Span<T> s(row, V);
+    const int hi = sp.hi(s.nb), ej = blockIdx.x == 0 ? s.edge(tid, V) : -1;
+    float w;
+    if (!row_live<OP>(a, r, y, w, blockIdx.x == 0)) {
+        for (int c = sp.lo(s.nb) + tid; c < hi; c += kSplitBlock) R::store(out + s.h + c * E, u32x4{0, 0, 0, 0});
+        if (ej >= 0) out[ej] = from_f32<T>(0.f);
+        return;
+    }
+    const RowToken<OP> token(a, r);
+    const MaxSum v = join_parts(sp, r);
+    const float zy = sp.zy[r];
+    if (tid == 0) coef = token.coef(a, r, w, (zy - v.m) - logf(v.s), blockIdx.x == 0);
+    __syncthreads();
+    const RowGrad<true> grad(RowExp<true>(v.m), a.cap, coef, v.s, 0.f);
+    for (int c = sp.lo(s.nb) + tid; c < hi; c += kSplitBlock) {
+        const u32x4 z = R::load(row + s.h + c * E);
+        float x[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = s.h + c * E + i == y ? grad.target(zy) : grad(R::get(z, i));
+        R::store(out + s.h + c * E, R::pack(x));
+    }
+    if (ej >= 0) out[ej] = from_f32<T>(ej == y ? grad.target(zy) : grad(to_f32<T>(row[ej])));
+}
+
+// Splitting reads the row twice and takes two launches: for long rows of which
+// there are too few to fill the card.  Unsplit and split, us a call (7 to 9 of
+// them the host's): gradient of 1, 64, 128 rows of 131072 bf16 values 18.5 9.7,
+// 21.3 13.5, 25.2 20.8; of 1, 128 of 65536 fp32 10.8 9.7, 17.9 18.8; the forward
+// of 3 rows of 131072 bf16 10.9 9.3, of 1 of 65536 fp32 7.7 9.6.
+constexpr int64_t kSplitRows = 128, kSplitValues = 65536, kPartChunks = 4 * kSplitBlock;
+int split_parts(LpOp op, int64_t n, int64_t V, int E) {
+    if (n > kSplitRows || V < kSplitValues + (op == LpOp::FWD)) return 1;
+    int64_t p = cdiv(cdiv(V, E), kPartChunks);
+    if (p > 1024 / n) p = 1024 / n;
+    return (int)(p > kWave ? kWave : p);
 }
 
 // Lanes and chunks per lane by the row's chunks.  Measured (fp32, TB/s of the
@@ -336,19 +454,48 @@ void launch_grad(hipStream_t st, const LpRows& a) {
 #undef AR_HELD
 }
 
+// The forward alone: TB/s of the rows read, by lanes: 8192 fp32 values 256 6.4,
+// 1024 2.7; 32768 bf16 256 6.0, 1024 4.6; 131072 bf16 256 5.6, 1024 6.0.
 template <typename T>
-int32_t launch(hipStream_t st, LpOp op, const LpRows& a, const char* nm) {
-    if (op == LpOp::FWD) lp_row_k<T, LpOp::FWD, 256><<<(unsigned)a.n, 256, 0, st>>>(a);
-    else if (op == LpOp::BWD) launch_grad<T, LpOp::BWD>(st, a);
-    else launch_grad<T, LpOp::POLICY>(st, a);
-    return check_launch(nm);
+void launch_fwd(hipStream_t st, const LpRows& a) {
+    const unsigned g = (unsigned)a.n;
+    const int64_t nc = cdiv(a.V, Row<T>::E);
+    if (nc <= 256) lp_row_k<T, LpOp::FWD, 64><<<g, 64, 0, st>>>(a);
+    else if (nc <= 8192 && a.n > 256) lp_row_k<T, LpOp::FWD, 256><<<g, 256, 0, st>>>(a);
+    else lp_row_k<T, LpOp::FWD, 1024><<<g, 1024, 0, st>>>(a);
+}
+
+template <typename T, LpOp OP>
+void launch_split(hipStream_t st, const LpRows& a, int parts) {
+    MaxSum* const part = static_cast<MaxSum*>(a.scratch);
+    const Split sp{part, reinterpret_cast<float*>(part + a.n * parts), parts};
+    const dim3 g(parts, (unsigned)a.n);
+    lp_part_k<T, OP><<<g, kSplitBlock, 0, st>>>(a, sp);
+    if constexpr (OP == LpOp::FWD) lp_join_k<<<(unsigned)a.n, kWave, 0, st>>>(a, sp);
+    else lp_apply_k<T, OP><<<g, kSplitBlock, 0, st>>>(a, sp);
+}
+
+template <typename T, LpOp OP>
+void launch(hipStream_t st, const LpRows& a) {
+    const int parts = a.scratch ? split_parts(OP, a.n, a.V, Row<T>::E) : 1;
+    if (parts > 1) launch_split<T, OP>(st, a, parts);
+    else if constexpr (OP == LpOp::FWD) launch_fwd<T>(st, a);
+    else launch_grad<T, OP>(st, a);
 }
 
 }  // namespace
 
+size_t lp_scratch(LpOp op, bool bf16_logits, int64_t n, int64_t V) {
+    const int parts = n > 0 ? split_parts(op, n, V, bf16_logits ? Row<bf16>::E : Row<float>::E) : 1;
+    return parts > 1 ? n * (parts * sizeof(MaxSum) + sizeof(float)) : 0;
+}
+
 int32_t lp_rows(hipStream_t st, LpOp op, bool bf16_logits, const LpRows& a, const char* nm) {
     if (a.n == 0) return AR_OK;
-    return bf16_logits ? launch<bf16>(st, op, a, nm) : launch<float>(st, op, a, nm);
+    if (op == LpOp::FWD) bf16_logits ? launch<bf16, LpOp::FWD>(st, a) : launch<float, LpOp::FWD>(st, a);
+    else if (op == LpOp::BWD) bf16_logits ? launch<bf16, LpOp::BWD>(st, a) : launch<float, LpOp::BWD>(st, a);
+    else bf16_logits ? launch<bf16, LpOp::POLICY>(st, a) : launch<float, LpOp::POLICY>(st, a);
+    return check_launch(nm);
 }
 
 int32_t check_rows(const char* nm, const void* logits, int32_t logits_bf16, const void* grad, const int64_t* targets,
@@ -370,10 +517,20 @@ int32_t check_rows(const char* nm, const void* logits, int32_t logits_bf16, cons
 
 using namespace ar;
 
+static int32_t rows_entry(ar_stream_t stream, LpOp op, bool bf16_logits, LpRows& a, const char* nm) {
+    if (const size_t bytes = lp_scratch(op, bf16_logits, a.n, a.V)) {
+        int32_t status;
+        a.scratch = workspace(S(stream), bytes, &status);
+        if (!a.scratch) return status;
+    }
+    return lp_rows(S(stream), op, bf16_logits, a, nm);
+}
+
 extern "C" int32_t ar_token_logprob_fwd(ar_stream_t stream, float* logp_out, const void* logits, int32_t logits_bf16,
                                         const int64_t* targets, int64_t num_tokens, int64_t vocab_size) {
     AR_CHECK_ARG(num_tokens <= 0 || logp_out, "token_logprob_fwd: null pointer");
-    if (const int32_t r = check_rows("token_logprob_fwd", logits, logits_bf16, nullptr, targets, num_tokens, vocab_size))
+    if (const int32_t r =
+            check_rows("token_logprob_fwd", logits, logits_bf16, nullptr, targets, num_tokens, vocab_size))
         return r;
     LpRows a;
     a.logits = logits;
@@ -381,7 +538,7 @@ extern "C" int32_t ar_token_logprob_fwd(ar_stream_t stream, float* logp_out, con
     a.logp = logp_out;
     a.n = num_tokens;
     a.V = vocab_size;
-    return lp_rows(S(stream), LpOp::FWD, logits_bf16 != 0, a, "token_logprob_fwd");
+    return rows_entry(stream, LpOp::FWD, logits_bf16 != 0, a, "token_logprob_fwd");
 }
 
 extern "C" int32_t ar_token_logprob_bwd(ar_stream_t stream, void* grad_logits, const void* logits, int32_t logits_bf16,
@@ -400,5 +557,5 @@ extern "C" int32_t ar_token_logprob_bwd(ar_stream_t stream, void* grad_logits, c
     a.cap = cap;
     a.n = num_tokens;
     a.V = vocab_size;
-    return lp_rows(S(stream), LpOp::BWD, logits_bf16 != 0, a, "token_logprob_bwd");
+    return rows_entry(stream, LpOp::BWD, logits_bf16 != 0, a, "token_logprob_bwd");
 }

@@ -505,15 +505,17 @@ struct PolicyWs {
     Totals* total;
     float* weight;
     double2* part;
+    char* rows;  // lp_rows' scratch
     size_t bytes;
 };
-PolicyWs policy_ws(char* base, const Seqs& q, int64_t nweights, int64_t nparts) {
+PolicyWs policy_ws(char* base, const Seqs& q, int64_t nweights, int64_t nparts, size_t row_bytes = 0) {
     Scratch s{base};
     PolicyWs w;
     w.cnt = s.take<int>(q.S * q.parts);
     w.total = s.take<Totals>(1);
     w.weight = s.take<float>(nweights);
     w.part = s.take<double2>(nparts);
+    w.rows = s.take<char>(row_bytes);
     w.bytes = s.used;
     return w;
 }
@@ -555,8 +557,10 @@ extern "C" int32_t ar_policy_loss(ar_stream_t stream, float* loss_out, float* gr
     if (!base) return status;
     const PolicyWs w = policy_ws(base, q, 0, blocks);
     const Totals* total = launch_counts(S(stream), q, w);
-    if (num_tokens / blocks > kTokBlock) policy_tokens_k<512><<<blocks, 512, 0, S(stream)>>>(q, w.cnt, total, a, w.part);
-    else policy_tokens_k<kTokBlock><<<blocks, kTokBlock, 0, S(stream)>>>(q, w.cnt, total, a, w.part);
+    if (num_tokens / blocks > kTokBlock)
+        policy_tokens_k<512><<<blocks, 512, 0, S(stream)>>>(q, w.cnt, total, a, w.part);
+    else
+        policy_tokens_k<kTokBlock><<<blocks, kTokBlock, 0, S(stream)>>>(q, w.cnt, total, a, w.part);
     sum_pairs_k<<<1, 1024, 0, S(stream)>>>(w.part, blocks, loss_out);
     return check_launch(nm);
 }
@@ -576,10 +580,12 @@ extern "C" int32_t ar_policy_loss_logits(ar_stream_t stream, float* loss_out, fl
                                        clip_high, kl_coef))
         return r;
     const Seqs q = policy_seqs(targets, seq_start, num_tokens, num_seqs, vocab_size);
+    const size_t row_bytes = lp_scratch(LpOp::POLICY, logits_bf16 != 0, num_tokens, vocab_size);
     int32_t status;
-    char* base = static_cast<char*>(workspace(S(stream), policy_ws(nullptr, q, num_tokens, num_tokens).bytes, &status));
+    char* base = static_cast<char*>(
+        workspace(S(stream), policy_ws(nullptr, q, num_tokens, num_tokens, row_bytes).bytes, &status));
     if (!base) return status;
-    const PolicyWs w = policy_ws(base, q, num_tokens, num_tokens);
+    const PolicyWs w = policy_ws(base, q, num_tokens, num_tokens, row_bytes);
     if (num_tokens <= kSmallTokens && num_seqs <= kSmallSeqs) {
         weight_small_k<<<1, kSmallBlock, 0, S(stream)>>>(q, per_seq, w.weight);
     } else {
@@ -594,6 +600,7 @@ extern "C" int32_t ar_policy_loss_logits(ar_stream_t stream, float* loss_out, fl
     a.logp = logp_out;
     a.weight = w.weight;
     a.terms = w.part;
+    a.scratch = row_bytes ? w.rows : nullptr;
     a.policy = PolicyIn{old_logp, ref_logp, advantages, 1.0 - clip_low, 1.0 + clip_high, kl_coef};
     a.cap = cap;
     a.loss_scale = loss_scale;

@@ -49,7 +49,9 @@ struct Row<bf16> {
     static __device__ __forceinline__ void store_nt(bf16* p, u32x4 v) {
         __builtin_nontemporal_store(v, reinterpret_cast<vec*>(p));
     }
-    static __device__ __forceinline__ u32x4 fill(float x) { return u32x4{1, 1, 1, 1} * (__float_as_uint(x) >> 16) * 0x10001u; }
+    static __device__ __forceinline__ u32x4 fill(float x) {
+        return u32x4{1, 1, 1, 1} * (__float_as_uint(x) >> 16) * 0x10001u;
+    }
 };
 
 // What one token adds to the policy loss, before its weight:
@@ -133,7 +135,9 @@ struct LpRows {
     float cap = 0.f;         // the softcap the logits went through, 0: none
     float loss_scale = 1.f;  // POLICY
     int64_t n = 0, V = 0;
+    void* scratch = nullptr;  // lp_scratch(...) bytes; null: no row is split
 };
+size_t lp_scratch(LpOp op, bool bf16_logits, int64_t n, int64_t V);
 int32_t lp_rows(hipStream_t st, LpOp op, bool bf16_logits, const LpRows& a, const char* nm);
 // What the entry points on logits check alike.
 int32_t check_rows(const char* nm, const void* logits, int32_t logits_bf16, const void* grad, const int64_t* targets,

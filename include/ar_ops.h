@@ -291,6 +291,8 @@ int32_t ar_muon_step(ar_stream_t stream, float* params, float* grads, float* mom
  * they are not read.  Sums over tokens are fp64, in a fixed order.
  *
  * num_tokens up to 2^31 - 1, vocab_size up to 2^30 (AR_EUNSUPPORTED above).
+ * Calls on up to 128 tokens with a vocabulary of 65536 or more take scratch
+ * from the workspace.
  * Arrays of no elements may be NULL. */
 
 /* logp_out[t] = z[t, targets[t]] - log sum_j exp(z[t, j]) */

@@ -95,6 +95,18 @@ SIZES = [1, 2, 3, 7, 8, 9, 255, 511, 512, 513, 1025, 2047, 2048, 2050, 8191, 819
 @pytest.mark.parametrize("V", SIZES + [131072, 131079, 270001])
 @pytest.mark.parametrize("n,off", [(19, 0), (2, 1)])
 def test_logprob_and_gradient(env, V, dtype, n, off):
+    check_logprob_and_gradient(env, V, dtype, n, off)
+
+
+# long rows that are many enough not to be split over workgroups
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("V", [32769, 65537, 131072, 131079, 150001])
+@pytest.mark.parametrize("n,off", [(128, 1), (129, 0), (131, 1)])
+def test_many_long_rows(env, V, dtype, n, off):
+    check_logprob_and_gradient(env, V, dtype, n, off)
+
+
+def check_logprob_and_gradient(env, V, dtype, n, off):
     torch, ops = env
     dt = getattr(torch, dtype)
     cap = 15.0 if V % 2 else 0.0
