@@ -63,22 +63,28 @@ __device__ __forceinline__ MaxSum block_max_sum(MaxSum v, float* red) {
     return t;
 }
 
-// A token's values for POLICY, loaded ahead of its row; nothing otherwise.
+// A token's values for POLICY, loaded ahead of its row; nothing otherwise.  The
+// row waits for coef, its gradient by logp (w: the token's weight or
+// gradient); what else the token has comes behind the row's last store, in one
+// lane (65536 rows of 8192 fp32 values: both before the row in fp64 798 us, in
+// fp32 725, so 713).
 template <LpOp OP>
 struct RowToken {
     __device__ __forceinline__ RowToken(const LpRows&, int64_t) {}
-    // The gradient by logp; w: the token's weight or gradient; out: write what else the token has.
-    __device__ __forceinline__ float coef(const LpRows&, int64_t, float w, float, bool) const { return w; }
+    __device__ __forceinline__ float coef(const LpRows&, float w, float) const { return w; }
+    __device__ __forceinline__ void finish(const LpRows&, int64_t, float, float) const {}
 };
 template <>
 struct RowToken<LpOp::POLICY> {
     PolicyToken t;
     __device__ __forceinline__ RowToken(const LpRows& a, int64_t r) : t(a.policy, r) {}
-    __device__ __forceinline__ float coef(const LpRows& a, int64_t r, float w, float logp, bool out) const {
+    __device__ __forceinline__ float coef(const LpRows& a, float w, float logp) const {
+        return w * policy_slope(logp, t, a.policy) * a.loss_scale;
+    }
+    __device__ __forceinline__ void finish(const LpRows& a, int64_t r, float w, float logp) const {
         const PolicyTerm<float> o = policy_term<float>(logp, t, a.policy);
-        if (out && a.logp) a.logp[r] = logp;
-        if (out) a.terms[r] = make_double2((double)w * o.loss, (double)w * o.kl);
-        return w * o.g * a.loss_scale;
+        if (a.logp) a.logp[r] = logp;
+        a.terms[r] = make_double2((double)w * o.loss, (double)w * o.kl);
     }
 };
 
@@ -208,7 +214,8 @@ __global__ __launch_bounds__(TB) void lp_row_k(LpRows a) {
         if (tid == 0) a.logp[r] = (zy - v.m) - logf(v.s);
         return;
     }
-    if (tid == 0) coef = token.coef(a, r, w, (zy - v.m) - logf(v.s), true);
+    const float logp = (zy - v.m) - logf(v.s);
+    if (tid == 0) coef = token.coef(a, w, logp);
     __syncthreads();  // zy and the sums are read: from here the row may be overwritten
     const RowGrad<true> grad(RowExp<true>(v.m), a.cap, coef, v.s, 0.f);
     auto emit = [&](int c, u32x4 z) {
@@ -225,18 +232,21 @@ __global__ __launch_bounds__(TB) void lp_row_k(LpRows a) {
     }
     for (int c = whole + tid; c < nb; c += TB) emit(c, R::load(row + h + c * E));
     if (ej >= 0) out[ej] = from_f32<T>(ej == y ? grad.target(zy) : grad(ez));
+    if (tid == 0) token.finish(a, r, w, logp);
 }
 
-// The same for rows of up to NV TB chunks of 16 bytes, held in registers: one
-// read, and the maximum before the exponentials.  Only rows with a chunk may
-// come to an instance with SURE > 0: its first SURE steps ask no question (the
-// row's last chunk is loaded where a lane has none, and not used).
-template <typename T, LpOp OP, int TB, int NV, int SURE>
-__global__ __launch_bounds__(TB, NV > 8 ? 4 : 8) void lp_held_k(LpRows a) {
+// The same for rows of up to (NV + NL) TB chunks of 16 bytes, held on the CU, NV
+// a lane in registers and NL in LDS: one read, and the maximum before the
+// exponentials.  Only rows with a chunk may come to an instance with SURE > 0:
+// its first SURE steps ask no question (the row's last chunk is loaded where a
+// lane has none, and not used).
+template <typename T, LpOp OP, int TB, int NV, int SURE, int NL = 0>
+__global__ __launch_bounds__(TB, NV > 9 ? 4 : 8) void lp_held_k(LpRows a) {
     using R = Row<T>;
-    constexpr int E = R::E;
+    constexpr int E = R::E, N = NV + NL;
     __shared__ float red[2 * (TB / kWave)];
     __shared__ float coef;
+    __shared__ u32x4 more[NL ? NL * TB : 1];  // lane t's: t, t + TB, ...
     const int64_t r = blockIdx.x;
     const int V = (int)a.V, tid = threadIdx.x;
     const int64_t y = a.targets[r];
@@ -248,24 +258,28 @@ __global__ __launch_bounds__(TB, NV > 8 ? 4 : 8) void lp_held_k(LpRows a) {
     const Span<T> sp(row, V);
     const int h = sp.h, nb = sp.nb;
     const u32x4 none = R::fill(-INFINITY);
-    u32x4 q[NV];
+    u32x4 q[N];  // from NV on only until they are in LDS
+    auto there = [&](int k) { return k < SURE || k * TB < nb; };
+    auto chunk = [&](int k) { return k < NV ? q[k] : more[(k - NV) * TB + tid]; };
+    auto keep = [&](int k, u32x4 v) {
+        if (k < NV) q[k] = v;
+        else more[(k - NV) * TB + tid] = v;
+    };
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-        if (k < SURE || k * TB < nb) {
-            const int c = tid + k * TB;
-            q[k] = R::load(row + h + min(c, nb - 1) * E);
-        }
+    for (int k = 0; k < N; ++k)
+        if (there(k)) q[k] = R::load(row + h + min(tid + k * TB, nb - 1) * E);
     const int ej = sp.edge(tid, V);
     float ez = ej >= 0 ? to_f32<T>(row[ej]) : -INFINITY;
     float zy = to_f32<T>(row[y]);
     float mt = ez;
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-        if (k < SURE || k * TB < nb) {
+    for (int k = 0; k < N; ++k)
+        if (there(k)) {
             if (tid + k * TB >= nb) q[k] = none;
 #pragma unroll
             for (int i = 0; i < E; ++i) mt = fmaxf(mt, R::get(q[k], i));
             again(q[k]);
+            if (k >= NV) keep(k, q[k]);
         }
     float m = block_max(mt, red);
     float z0 = 0.f;
@@ -273,13 +287,15 @@ __global__ __launch_bounds__(TB, NV > 8 ? 4 : 8) void lp_held_k(LpRows a) {
         // the same in every lane: shorten the row by its maximum.  (Values
         // that bf16 rounds here differ from it by 2^12 or more: no weight.)
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            float x[E];
+        for (int k = 0; k < N; ++k)
+            if (there(k)) {
+                const u32x4 v = chunk(k);
+                float x[E];
 #pragma unroll
-            for (int i = 0; i < E; ++i) x[i] = R::get(q[k], i) - m;
-            q[k] = R::pack(x);
-            again(q[k]);
-        }
+                for (int i = 0; i < E; ++i) x[i] = R::get(v, i) - m;
+                keep(k, R::pack(x));
+                if (k < NV) again(q[k]);
+            }
         ez -= m;
         zy -= m;
         z0 = m;
@@ -288,26 +304,29 @@ __global__ __launch_bounds__(TB, NV > 8 ? 4 : 8) void lp_held_k(LpRows a) {
     const RowExp<false> ex(m);
     float st = ex(ez);
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-        if (k < SURE || k * TB < nb) {
+    for (int k = 0; k < N; ++k)
+        if (there(k)) {
+            const u32x4 v = chunk(k);
             float s = 0.f;
 #pragma unroll
-            for (int i = 0; i < E; ++i) s += ex(R::get(q[k], i));
+            for (int i = 0; i < E; ++i) s += ex(R::get(v, i));
             st += s;
-            again(q[k]);
+            if (k < NV) again(q[k]);
         }
     st = block_sum(st, red + TB / kWave);
-    if (tid == 0) coef = token.coef(a, r, w, ex.logp(zy, st), true);
+    const float logp = ex.logp(zy, st);
+    if (tid == 0) coef = token.coef(a, w, logp);
     __syncthreads();
     const RowGrad<false> grad(ex, a.cap, coef, st, z0);
     const int yc = y < h ? -1 : ((int)y - h) / E, yi = y < h ? 0 : ((int)y - h) % E;
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-        if (k < SURE || k * TB < nb) {
+    for (int k = 0; k < N; ++k)
+        if (there(k)) {
             const int c = tid + k * TB;
+            const u32x4 v = chunk(k);
             float x[E];
 #pragma unroll
-            for (int i = 0; i < E; ++i) x[i] = grad(R::get(q[k], i));
+            for (int i = 0; i < E; ++i) x[i] = grad(R::get(v, i));
             if (c == yc) {
                 const float t = grad.target(zy);
 #pragma unroll
@@ -316,6 +335,7 @@ __global__ __launch_bounds__(TB, NV > 8 ? 4 : 8) void lp_held_k(LpRows a) {
             if (c < nb) R::store(out + h + c * E, R::pack(x));
         }
     if (ej >= 0) out[ej] = from_f32<T>(ej == y ? grad.target(zy) : grad(ez));
+    if (tid == 0) token.finish(a, r, w, logp);
 }
 
 // ---- few long rows: each split over several workgroups ----
@@ -404,7 +424,8 @@ __global__ __launch_bounds__(kSplitBlock) void lp_apply_k(LpRows a, Split sp) {
     const RowToken<OP> token(a, r);
     const MaxSum v = join_parts(sp, r);
     const float zy = sp.zy[r];
-    if (tid == 0) coef = token.coef(a, r, w, (zy - v.m) - logf(v.s), blockIdx.x == 0);
+    const float logp = (zy - v.m) - logf(v.s);
+    if (tid == 0) coef = token.coef(a, w, logp);
     __syncthreads();
     const RowGrad<true> grad(RowExp<true>(v.m), a.cap, coef, v.s, 0.f);
     for (int c = sp.lo(s.nb) + tid; c < hi; c += kSplitBlock) {
@@ -415,6 +436,7 @@ __global__ __launch_bounds__(kSplitBlock) void lp_apply_k(LpRows a, Split sp) {
         R::store(out + s.h + c * E, R::pack(x));
     }
     if (ej >= 0) out[ej] = from_f32<T>(ej == y ? grad.target(zy) : grad(to_f32<T>(row[ej])));
+    if (tid == 0 && blockIdx.x == 0) token.finish(a, r, w, logp);
 }
 
 // Splitting reads the row twice and takes two launches: for long rows of which
@@ -430,18 +452,21 @@ int split_parts(LpOp op, int64_t n, int64_t V, int E) {
     return (int)(p > kWave ? kWave : p);
 }
 
-// Lanes and chunks per lane by the row's chunks.  Measured (fp32, TB/s of the
-// row read and the gradient written): with as few chunks per lane as 1024 lanes
-// allow, down to two, a row is in flight the shortest: 8192 values 1024 x 2 6.1,
-// 512 x 4 5.4, 256 x 8 5.5; 16384 values 1024 x 4 6.0, 512 x 8 5.3.  bf16 has
-// twice the values per chunk and takes four: 8192 values 256 x 4 5.8, 512 x 2
-// 5.6, 1024 x 1 3.7.
+// Lanes and chunks per lane by the row's chunks (TB/s of the row read and the
+// gradient written).  With as few chunks per lane as 1024 lanes allow, down to
+// two, a row is in flight the shortest: 8192 fp32 values 1024 x 2 6.1, 512 x 4
+// 5.4, 256 x 8 5.5; 16384 1024 x 4 6.0, 512 x 8 5.3.  bf16 has twice the values
+// per chunk and takes four: 8192 values 256 x 4 5.8, 512 x 2 5.6, 1024 x 1 3.7.
+// Two workgroups of 1024 fit a CU with up to 64 registers and 80 KiB of LDS
+// each, one with more, whose reads, sums and writes then take turns: 90000 bf16
+// values 8 chunks in registers and 4 in LDS 5.0, 16 in registers 4.6; 131072
+// 4.8 (bound by arithmetic: fp32 rows of those bytes 5.3); 50001 fp32 5.0, 4.7.
 template <typename T, LpOp OP>
 void launch_grad(hipStream_t st, const LpRows& a) {
     const unsigned g = (unsigned)a.n;
     const int64_t nc = cdiv(a.V, Row<T>::E);
 #define AR_HELD(TB, NV) lp_held_k<T, OP, TB, NV, NV / 2><<<g, TB, 0, st>>>(a)
-    constexpr int M = sizeof(T) == 2 ? 4 : 2;
+    constexpr int M = sizeof(T) == 2 ? 4 : 2, HR = sizeof(T) == 2 ? 8 : 9;
     if (nc <= 64 * 2) lp_held_k<T, OP, 64, 2, 0><<<g, 64, 0, st>>>(a);  // rows without a whole chunk too
     else if (nc <= 128 * M) AR_HELD(128, M);
     else if (nc <= 256 * M) AR_HELD(256, M);
@@ -449,6 +474,7 @@ void launch_grad(hipStream_t st, const LpRows& a) {
     else if (nc <= 1024 * M) AR_HELD(1024, M);
     else if (nc <= 1024 * 4) AR_HELD(1024, 4);
     else if (nc <= 1024 * 8) AR_HELD(1024, 8);
+    else if (nc <= 1024 * (HR + 4)) lp_held_k<T, OP, 1024, HR, 8, 4><<<g, 1024, 0, st>>>(a);
     else if (nc <= 1024 * 16) AR_HELD(1024, 16);
     else lp_row_k<T, OP, 1024><<<g, 1024, 0, st>>>(a);
 #undef AR_HELD

@@ -206,8 +206,8 @@ __global__ __launch_bounds__(TB) void policy_tokens_k(Seqs q, const int* cnt, co
 // ---- small batches: one block ----
 // The sequences' offsets, their counts and the tokens' sequences in LDS.
 constexpr int kSmallBlock = 1024, kSmallSeqs = 1024;
-constexpr int kSmallTokens = 8192;  // weights, pairs; the policy loss with its fp64 exponentials:
-constexpr int kSmallPolicy = 2048;  // 8.4 us at 500 tokens, 10.2 at 2048, 15.0 at 4000 (three launches: 13.8)
+constexpr int kSmallTokens = 8192;  // pairs: 12.8 us at 8000, three launches 13.2
+constexpr int kSmallPolicy = 2048;  // policy loss: 8.4 us at 500, 10.2 at 2048, 15.0 at 4000, three launches 13.8
 struct SmallSeqs {
     int start[kSmallSeqs + 1], cnt[kSmallSeqs];
     int16_t seq[kSmallTokens];  // -1: the token does not count
@@ -280,21 +280,42 @@ __global__ __launch_bounds__(kSmallBlock) void policy_small_k(Seqs q, PolicyToke
     }
 }
 
-// out[0], out[1] = the sums of part's n pairs, in a fixed order.
-__global__ __launch_bounds__(1024) void sum_pairs_k(const double2* part, int64_t n, float* out) {
+// The sums of a block's kSumPairs of part's n pairs, in a fixed order: to out
+// (n <= kSumPairs), or to part2 for another such launch.  One block for all of
+// 65536 pairs took 36 us, with eight loads in flight 23, in two launches 11.
+constexpr int64_t kSumPairs = 4096;
+__global__ __launch_bounds__(1024) void sum_pairs_k(const double2* part, int64_t n, double2* part2, float* out) {
     __shared__ double red[16];
     double a = 0.0, b = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
-        const double2 v = part[i];
+#pragma unroll
+    for (int k = 0; k < kSumPairs / 1024; ++k) {
+        const int64_t i = blockIdx.x * kSumPairs + threadIdx.x + k * 1024;
+        const double2 v = i < n ? part[i] : make_double2(0.0, 0.0);
         a += v.x;
         b += v.y;
     }
     a = block_total(a, red);
     b = block_total(b, red);
     if (threadIdx.x == 0) {
-        out[0] = (float)a;
-        out[1] = (float)b;
+        if (part2) {
+            part2[blockIdx.x] = make_double2(a, b);
+        } else {
+            out[0] = (float)a;
+            out[1] = (float)b;
+        }
     }
+}
+
+// How many pairs sum_pairs needs, for the sums of sums behind the n.
+int64_t pair_room(int64_t n) {
+    int64_t room = n;
+    while (n > kSumPairs) room += n = cdiv(n, kSumPairs);
+    return room;
+}
+void sum_pairs(hipStream_t st, double2* part, int64_t n, float* out) {
+    for (; n > kSumPairs; part += n, n = cdiv(n, kSumPairs))
+        sum_pairs_k<<<(unsigned)cdiv(n, kSumPairs), 1024, 0, st>>>(part, n, part + n, nullptr);
+    sum_pairs_k<<<1, 1024, 0, st>>>(part, n, nullptr, out);
 }
 
 // ---- preference ----
@@ -514,7 +535,7 @@ PolicyWs policy_ws(char* base, const Seqs& q, int64_t nweights, int64_t nparts, 
     w.cnt = s.take<int>(q.S * q.parts);
     w.total = s.take<Totals>(1);
     w.weight = s.take<float>(nweights);
-    w.part = s.take<double2>(nparts);
+    w.part = s.take<double2>(pair_room(nparts));
     w.rows = s.take<char>(row_bytes);
     w.bytes = s.used;
     return w;
@@ -561,7 +582,7 @@ extern "C" int32_t ar_policy_loss(ar_stream_t stream, float* loss_out, float* gr
         policy_tokens_k<512><<<blocks, 512, 0, S(stream)>>>(q, w.cnt, total, a, w.part);
     else
         policy_tokens_k<kTokBlock><<<blocks, kTokBlock, 0, S(stream)>>>(q, w.cnt, total, a, w.part);
-    sum_pairs_k<<<1, 1024, 0, S(stream)>>>(w.part, blocks, loss_out);
+    sum_pairs(S(stream), w.part, blocks, loss_out);
     return check_launch(nm);
 }
 
@@ -586,7 +607,7 @@ extern "C" int32_t ar_policy_loss_logits(ar_stream_t stream, float* loss_out, fl
         workspace(S(stream), policy_ws(nullptr, q, num_tokens, num_tokens, row_bytes).bytes, &status));
     if (!base) return status;
     const PolicyWs w = policy_ws(base, q, num_tokens, num_tokens, row_bytes);
-    if (num_tokens <= kSmallTokens && num_seqs <= kSmallSeqs) {
+    if (num_tokens <= kSmallPolicy && num_seqs <= kSmallSeqs) {
         weight_small_k<<<1, kSmallBlock, 0, S(stream)>>>(q, per_seq, w.weight);
     } else {
         const Totals* total = launch_counts(S(stream), q, w);
@@ -607,7 +628,7 @@ extern "C" int32_t ar_policy_loss_logits(ar_stream_t stream, float* loss_out, fl
     a.n = num_tokens;
     a.V = vocab_size;
     if (const int32_t r = lp_rows(S(stream), LpOp::POLICY, logits_bf16 != 0, a, nm)) return r;
-    sum_pairs_k<<<1, 1024, 0, S(stream)>>>(w.part, num_tokens, loss_out);
+    sum_pairs(S(stream), w.part, num_tokens, loss_out);
     return check_launch(nm);
 }
 

@@ -61,10 +61,8 @@ struct Row<bf16> {
 // A < 0; there pg does not depend on logp.
 // F = double where log-probabilities are given: the difference of two fp32
 // values is exact in it, and r meets the bounds unrounded.  F = float where
-// they come out of a row of logits: what fp32 adds to their own error (a few
-// 1e-7) is less, and one lane's fp64 exponentials held up the row (65536 rows
-// of 8192 fp32 values: 798 us, in fp32 and with the token's values loaded
-// ahead 725).
+// they come out of a row of logits, to which it adds less than their own error
+// (a few 1e-7).
 struct PolicyIn {
     const float *old_logp, *ref_logp, *adv;  // old_logp null: old = logp; ref_logp null: no KL term
     double lo, hi, kl_coef;
@@ -97,6 +95,16 @@ __device__ __forceinline__ PolicyTerm<F> policy_term(F logp, const PolicyToken& 
         }
     }
     return o;
+}
+
+// g alone, in fp32 with the hardware's exponential.
+__device__ __forceinline__ float policy_slope(float logp, const PolicyToken& t, const PolicyIn& in) {
+    constexpr float kL2e = 1.44269504f;
+    const float a = t.adv, r = in.old_logp ? __builtin_amdgcn_exp2f((logp - t.old_logp) * kL2e) : 1.f;
+    float g = (a > 0.f && r > (float)in.hi) || (a < 0.f && r < (float)in.lo) ? 0.f : -a * r;
+    if (in.ref_logp && in.kl_coef != 0.0)
+        g -= (float)in.kl_coef * (__builtin_amdgcn_exp2f((t.ref_logp - logp) * kL2e) - 1.f);
+    return g;
 }
 
 __device__ __forceinline__ double wave_sum(double v) {
