@@ -9,6 +9,8 @@
 // pass) and a row of the gradient written once.
 #include <math.h>
 
+#include <algorithm>
+
 #include "ar_losses.hpp"
 
 namespace ar {
@@ -185,7 +187,7 @@ __global__ __launch_bounds__(TB) void lp_row_k(LpRows a) {
     constexpr int E = R::E;
     __shared__ float red[2 * (TB / kWave)];
     __shared__ float coef;
-    const int64_t r = blockIdx.x;
+    const int64_t r = a.first + blockIdx.x;
     const int V = (int)a.V, tid = threadIdx.x;
     const int64_t y = a.targets[r];
     const T* row = static_cast<const T*>(a.logits) + r * a.V;
@@ -247,7 +249,7 @@ __global__ __launch_bounds__(TB, NV > 9 ? 4 : 8) void lp_held_k(LpRows a) {
     __shared__ float red[2 * (TB / kWave)];
     __shared__ float coef;
     __shared__ u32x4 more[NL ? NL * TB : 1];  // lane t's: t, t + TB, ...
-    const int64_t r = blockIdx.x;
+    const int64_t r = a.first + blockIdx.x;
     const int V = (int)a.V, tid = threadIdx.x;
     const int64_t y = a.targets[r];
     const T* row = static_cast<const T*>(a.logits) + r * a.V;
@@ -462,8 +464,7 @@ int split_parts(LpOp op, int64_t n, int64_t V, int E) {
 // values 8 chunks in registers and 4 in LDS 5.0, 16 in registers 4.6; 131072
 // 4.8 (bound by arithmetic: fp32 rows of those bytes 5.3); 50001 fp32 5.0, 4.7.
 template <typename T, LpOp OP>
-void launch_grad(hipStream_t st, const LpRows& a) {
-    const unsigned g = (unsigned)a.n;
+void launch_grad(hipStream_t st, const LpRows& a, unsigned g) {
     const int64_t nc = cdiv(a.V, Row<T>::E);
 #define AR_HELD(TB, NV) lp_held_k<T, OP, TB, NV, NV / 2><<<g, TB, 0, st>>>(a)
     constexpr int M = sizeof(T) == 2 ? 4 : 2, HR = sizeof(T) == 2 ? 8 : 9;
@@ -483,8 +484,7 @@ void launch_grad(hipStream_t st, const LpRows& a) {
 // The forward alone: TB/s of the rows read, by lanes: 8192 fp32 values 256 6.4,
 // 1024 2.7; 32768 bf16 256 6.0, 1024 4.6; 131072 bf16 256 5.6, 1024 6.0.
 template <typename T>
-void launch_fwd(hipStream_t st, const LpRows& a) {
-    const unsigned g = (unsigned)a.n;
+void launch_fwd(hipStream_t st, const LpRows& a, unsigned g) {
     const int64_t nc = cdiv(a.V, Row<T>::E);
     if (nc <= 256) lp_row_k<T, LpOp::FWD, 64><<<g, 64, 0, st>>>(a);
     else if (nc <= 8192 && a.n > 256) lp_row_k<T, LpOp::FWD, 256><<<g, 256, 0, st>>>(a);
@@ -504,9 +504,15 @@ void launch_split(hipStream_t st, const LpRows& a, int parts) {
 template <typename T, LpOp OP>
 void launch(hipStream_t st, const LpRows& a) {
     const int parts = a.scratch ? split_parts(OP, a.n, a.V, Row<T>::E) : 1;
-    if (parts > 1) launch_split<T, OP>(st, a, parts);
-    else if constexpr (OP == LpOp::FWD) launch_fwd<T>(st, a);
-    else launch_grad<T, OP>(st, a);
+    if (parts > 1) return launch_split<T, OP>(st, a, parts);
+    // a launch holds fewer than 2^32 lanes: 2^22 rows of 1024
+    constexpr int64_t kRows = 1 << 21;
+    LpRows part = a;
+    for (part.first = 0; part.first < a.n; part.first += kRows) {
+        const unsigned rows = (unsigned)std::min(kRows, a.n - part.first);
+        if constexpr (OP == LpOp::FWD) launch_fwd<T>(st, part, rows);
+        else launch_grad<T, OP>(st, part, rows);
+    }
 }
 
 }  // namespace

@@ -14,7 +14,7 @@ namespace ar {
 namespace {
 
 constexpr int kTokBlock = 256;
-constexpr int64_t kMaxItems = 2048;    // sequences x parts, where sequences are split
+constexpr int64_t kMaxItems = 2048;     // sequences x parts, where sequences are split
 constexpr int64_t kInlineItems = 1024;  // counts that every block adds up itself
 
 struct Seqs {
@@ -25,7 +25,7 @@ struct Seqs {
 
 // Tokens of an item.  Offsets outside [0, n], or descending ones, give
 // shortened or empty sequences, never an access out of range.
-// (All in 32 bits: at most 2^31 - 1 tokens, 2^30 sequences.)
+// (Divisions in 32 bits: at most 2^31 - 1 tokens, 2^30 sequences.)
 __device__ __forceinline__ uint32_t item_seq(const Seqs& q, int64_t item) { return (uint32_t)item / (uint32_t)q.parts; }
 __device__ __forceinline__ void item_range(const Seqs& q, int64_t item, int64_t& lo, int64_t& hi) {
     const uint32_t s = item_seq(q, item), p = (uint32_t)item - s * q.parts;
@@ -171,8 +171,8 @@ struct Token {
 // exponentials behind it, not by bytes: 262144 tokens of 509 sequences (6.5 MB)
 // 10.4 us, 8.4 of them without the counts (which would take a launch of 3.7).
 template <int TB>
-__global__ __launch_bounds__(TB) void policy_tokens_k(Seqs q, const int* cnt, const Totals* total,
-                                                             PolicyTokens a, double2* part) {
+__global__ __launch_bounds__(TB) void policy_tokens_k(Seqs q, const int* cnt, const Totals* total, PolicyTokens a,
+                                                      double2* part) {
     __shared__ double red[TB / kWave];
     __shared__ TotalsLds l;
     double loss = 0.0, kl = 0.0;
@@ -479,8 +479,7 @@ Seqs make_seqs(const int64_t* targets, const int64_t* start, int64_t n, int64_t 
     if (parts < 1) parts = 1;
     return Seqs{targets, start, n, S, V, (int)parts};
 }
-// A token is a few loads and two exponentials in turn: one per lane, where the
-// sequences are few enough.
+// A lane takes its tokens in turn: parts of a few per lane.
 Seqs policy_seqs(const int64_t* targets, const int64_t* start, int64_t n, int64_t S, int64_t V) {
     return make_seqs(targets, start, n, S, V, 1024, kMaxItems);
 }

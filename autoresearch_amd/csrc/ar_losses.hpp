@@ -142,7 +142,7 @@ struct LpRows {
     PolicyIn policy{};
     float cap = 0.f;         // the softcap the logits went through, 0: none
     float loss_scale = 1.f;  // POLICY
-    int64_t n = 0, V = 0;
+    int64_t n = 0, V = 0, first = 0;  // first: a launch's first row
     void* scratch = nullptr;  // lp_scratch(...) bytes; null: no row is split
 };
 size_t lp_scratch(LpOp op, bool bf16_logits, int64_t n, int64_t V);

@@ -287,8 +287,8 @@ int32_t ar_muon_step(ar_stream_t stream, float* params, float* grads, float* mom
  * it lies in one: sequence s holds tokens seq_start[s] .. seq_start[s + 1] - 1
  * (device, num_seqs + 1 ascending offsets in [0, num_tokens]; with others, which
  * tokens count is not defined, but nothing outside the arrays is touched).  A token that does not count has
- * log-probability 0 and gradient 0, whatever its logits or other inputs hold:
- * they are not read.  Sums over tokens are fp64, in a fixed order.
+ * log-probability 0 and gradient 0, whatever its logits or other inputs hold;
+ * its logits are not read.  Sums over tokens are fp64, in a fixed order.
  *
  * num_tokens up to 2^31 - 1, vocab_size up to 2^30 (AR_EUNSUPPORTED above).
  * Calls on up to 128 tokens with a vocabulary of 65536 or more take scratch

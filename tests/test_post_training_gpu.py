@@ -106,6 +106,20 @@ def test_many_long_rows(env, V, dtype, n, off):
     check_logprob_and_gradient(env, V, dtype, n, off)
 
 
+def test_more_rows_than_a_launch_holds(env):
+    torch, ops = env
+    n, V = (1 << 21) + 3, 5
+    g = gen(torch, 3)
+    z, y = torch.randn(n, V, generator=g, device="cuda"), torch.randint(0, V, (n,), generator=g, device="cuda")
+    logp, out = torch.empty(n, device="cuda"), torch.empty_like(z)
+    ops.token_logprob_fwd(logp, z, y, n, V)
+    ops.token_logprob_bwd(out, z, y, torch.ones(n, device="cuda"), 0.0, n, V)
+    want, p, lse, m, z_y, ok = ref_rows(torch, z, y)
+    close(torch, logp, want, logp_tol(V, z_y, m, lse, want), torch.float32)
+    d, tol = ref_grad(torch, z, y, p, ok, torch.ones(n, device="cuda"), 0.0)
+    close(torch, out, d, tol, torch.float32)
+
+
 def check_logprob_and_gradient(env, V, dtype, n, off):
     torch, ops = env
     dt = getattr(torch, dtype)
