@@ -33,6 +33,50 @@ struct Span {
     }
 };
 
+// Reductions over a wave without LDS: lanes to the left within rows of 16 (row
+// shift 1, 2, 4, 8), then rows to the right of them (broadcasts of lane 15 and
+// 31), `none` where there is no lane; the last lane's result to all.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ float dpp(float none, float v) {
+    return __int_as_float(
+        __builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+struct Max {
+    static constexpr float none = -INFINITY;
+    static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); }
+};
+struct Sum {
+    static constexpr float none = 0.f;
+    static __device__ __forceinline__ float of(float a, float b) { return a + b; }
+};
+template <typename O>
+__device__ __forceinline__ float of_row16(float v) {  // lane 15 of each row
+    v = O::of(v, dpp<0x111>(O::none, v));
+    v = O::of(v, dpp<0x112>(O::none, v));
+    v = O::of(v, dpp<0x114>(O::none, v));
+    return O::of(v, dpp<0x118>(O::none, v));
+}
+__device__ __forceinline__ float lane_value(float v, int lane) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+template <typename O>
+__device__ __forceinline__ float of_wave(float v) {
+    v = of_row16<O>(v);
+    v = O::of(v, dpp<0x142, 0xa>(O::none, v));
+    return lane_value(O::of(v, dpp<0x143, 0xc>(O::none, v)), 63);
+}
+// Over a block of up to 16 waves; red: a value per wave that nothing else of
+// the kernel uses.  One barrier.
+template <typename O>
+__device__ __forceinline__ float of_block(float v, float* red) {
+    v = of_wave<O>(v);
+    const int lane = threadIdx.x % kWave, nw = blockDim.x / kWave;
+    if (nw == 1) return v;
+    if (lane == 0) red[threadIdx.x / kWave] = v;
+    __syncthreads();
+    return lane_value(of_row16<O>(lane < nw ? red[lane] : O::none), 15);
+}
+
 // The maximum so far and the sum of exp(z - m) under it.
 struct MaxSum {
     float m = -INFINITY, s = 0.f;
@@ -45,23 +89,32 @@ struct MaxSum {
         s = s * __expf(m - nm) + os * __expf(om - nm);
         m = nm;
     }
+    // the same sum under another maximum (-inf: of nothing)
+    __device__ __forceinline__ float under(float nm) const { return s * __expf(m - (nm == -INFINITY ? 0.f : nm)); }
 };
+__device__ __forceinline__ MaxSum wave_max_sum(MaxSum v) {
+    MaxSum t;
+    t.m = of_wave<Max>(v.m);
+    t.s = of_wave<Sum>(v.under(t.m));
+    return t;
+}
+// red: two values per wave.
 __device__ __forceinline__ MaxSum block_max_sum(MaxSum v, float* red) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const float om = __shfl_xor(v.m, o, kWave), os = __shfl_xor(v.s, o, kWave);
-        v.add(om, os);
-    }
-    const int w = threadIdx.x / kWave, nw = blockDim.x / kWave;
+    v = wave_max_sum(v);
+    const int w = threadIdx.x / kWave, lane = threadIdx.x % kWave, nw = blockDim.x / kWave;
     if (nw == 1) return v;
-    __syncthreads();
-    if (threadIdx.x % kWave == 0) {
+    if (lane == 0) {
         red[2 * w] = v.m;
         red[2 * w + 1] = v.s;
     }
     __syncthreads();
-    MaxSum t;
-    for (int i = 0; i < nw; ++i) t.add(red[2 * i], red[2 * i + 1]);
+    MaxSum o, t;
+    if (lane < nw) {
+        o.m = red[2 * lane];
+        o.s = red[2 * lane + 1];
+    }
+    t.m = lane_value(of_row16<Max>(o.m), 15);
+    t.s = lane_value(of_row16<Sum>(o.under(t.m)), 15);
     return t;
 }
 
@@ -186,7 +239,6 @@ __global__ __launch_bounds__(TB) void lp_row_k(LpRows a) {
     using R = Row<T>;
     constexpr int E = R::E;
     __shared__ float red[2 * (TB / kWave)];
-    __shared__ float coef;
     const int64_t r = a.first + blockIdx.x;
     const int V = (int)a.V, tid = threadIdx.x;
     const int64_t y = a.targets[r];
@@ -216,10 +268,9 @@ __global__ __launch_bounds__(TB) void lp_row_k(LpRows a) {
         if (tid == 0) a.logp[r] = (zy - v.m) - logf(v.s);
         return;
     }
+    // (all have read zy: from here the row may be overwritten)
     const float logp = (zy - v.m) - logf(v.s);
-    if (tid == 0) coef = token.coef(a, w, logp);
-    __syncthreads();  // zy and the sums are read: from here the row may be overwritten
-    const RowGrad<true> grad(RowExp<true>(v.m), a.cap, coef, v.s, 0.f);
+    const RowGrad<true> grad(RowExp<true>(v.m), a.cap, token.coef(a, w, logp), v.s, 0.f);
     auto emit = [&](int c, u32x4 z) {
         float x[E];
 #pragma unroll
@@ -247,7 +298,6 @@ __global__ __launch_bounds__(TB, NV > 9 ? 4 : 8) void lp_held_k(LpRows a) {
     using R = Row<T>;
     constexpr int E = R::E, N = NV + NL;
     __shared__ float red[2 * (TB / kWave)];
-    __shared__ float coef;
     __shared__ u32x4 more[NL ? NL * TB : 1];  // lane t's: t, t + TB, ...
     const int64_t r = a.first + blockIdx.x;
     const int V = (int)a.V, tid = threadIdx.x;
@@ -283,7 +333,7 @@ __global__ __launch_bounds__(TB, NV > 9 ? 4 : 8) void lp_held_k(LpRows a) {
             again(q[k]);
             if (k >= NV) keep(k, q[k]);
         }
-    float m = block_max(mt, red);
+    float m = of_block<Max>(mt, red);
     float z0 = 0.f;
     if (__builtin_amdgcn_readfirstlane(!(fabsf(m) < kFar))) {
         // the same in every lane: shorten the row by its maximum.  (Values
@@ -315,11 +365,9 @@ __global__ __launch_bounds__(TB, NV > 9 ? 4 : 8) void lp_held_k(LpRows a) {
             st += s;
             if (k < NV) again(q[k]);
         }
-    st = block_sum(st, red + TB / kWave);
+    st = of_block<Sum>(st, red + TB / kWave);
     const float logp = ex.logp(zy, st);
-    if (tid == 0) coef = token.coef(a, w, logp);
-    __syncthreads();
-    const RowGrad<false> grad(ex, a.cap, coef, st, z0);
+    const RowGrad<false> grad(ex, a.cap, token.coef(a, w, logp), st, z0);
     const int yc = y < h ? -1 : ((int)y - h) / E, yi = y < h ? 0 : ((int)y - h) % E;
 #pragma unroll
     for (int k = 0; k < N; ++k)
@@ -391,12 +439,7 @@ __device__ __forceinline__ MaxSum join_parts(const Split& sp, int64_t r) {
     const int lane = threadIdx.x % kWave;
     MaxSum v;
     if (lane < sp.parts) v = sp.part[r * sp.parts + lane];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const float om = __shfl_xor(v.m, o, kWave), os = __shfl_xor(v.s, o, kWave);
-        v.add(om, os);
-    }
-    return v;
+    return wave_max_sum(v);
 }
 __global__ __launch_bounds__(kWave) void lp_join_k(LpRows a, Split sp) {
     const int64_t r = blockIdx.x;
@@ -409,7 +452,6 @@ template <typename T, LpOp OP>
 __global__ __launch_bounds__(kSplitBlock) void lp_apply_k(LpRows a, Split sp) {
     using R = Row<T>;
     constexpr int E = R::E;
-    __shared__ float coef;
     const int64_t r = blockIdx.y;
     const int V = (int)a.V, tid = threadIdx.x;
     const int64_t y = a.targets[r];
@@ -427,9 +469,7 @@ __global__ __launch_bounds__(kSplitBlock) void lp_apply_k(LpRows a, Split sp) {
     const MaxSum v = join_parts(sp, r);
     const float zy = sp.zy[r];
     const float logp = (zy - v.m) - logf(v.s);
-    if (tid == 0) coef = token.coef(a, w, logp);
-    __syncthreads();
-    const RowGrad<true> grad(RowExp<true>(v.m), a.cap, coef, v.s, 0.f);
+    const RowGrad<true> grad(RowExp<true>(v.m), a.cap, token.coef(a, w, logp), v.s, 0.f);
     for (int c = sp.lo(s.nb) + tid; c < hi; c += kSplitBlock) {
         const u32x4 z = R::load(row + s.h + c * E);
         float x[E];
@@ -481,13 +521,15 @@ void launch_grad(hipStream_t st, const LpRows& a, unsigned g) {
 #undef AR_HELD
 }
 
-// The forward alone: TB/s of the rows read, by lanes: 8192 fp32 values 256 6.4,
-// 1024 2.7; 32768 bf16 256 6.0, 1024 4.6; 131072 bf16 256 5.6, 1024 6.0.
+// The forward alone: TB/s of the rows read, by lanes: 1024 bf16 values 64 5.7,
+// 256 2.4; 8192 bf16 256 6.4, 1024 3.2; 8192 fp32 256 6.4, 1024 5.2; 32768 bf16
+// 256 6.1, 1024 6.4; 150001 fp32 256 5.8, 1024 6.2.  Few rows: as many lanes as
+// a workgroup has.
 template <typename T>
 void launch_fwd(hipStream_t st, const LpRows& a, unsigned g) {
     const int64_t nc = cdiv(a.V, Row<T>::E);
     if (nc <= 256) lp_row_k<T, LpOp::FWD, 64><<<g, 64, 0, st>>>(a);
-    else if (nc <= 8192 && a.n > 256) lp_row_k<T, LpOp::FWD, 256><<<g, 256, 0, st>>>(a);
+    else if (nc <= 2048 && a.n > 256) lp_row_k<T, LpOp::FWD, 256><<<g, 256, 0, st>>>(a);
     else lp_row_k<T, LpOp::FWD, 1024><<<g, 1024, 0, st>>>(a);
 }
 
