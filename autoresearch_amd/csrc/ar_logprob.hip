@@ -233,67 +233,52 @@ __device__ __forceinline__ void again(u32x4& q) { asm volatile("" : "+v"(q)); }
 
 constexpr int kBatch = 4;  // chunks a lane has in flight
 
-// Rows of any length: the row is read again for the gradient.
-template <typename T, LpOp OP, int TB>
-__global__ __launch_bounds__(TB) void lp_row_k(LpRows a) {
+// The maximum and sum of a row's chunks [lo, hi), lane t's lo + t, lo + t + TB, ...
+template <typename T, int TB>
+__device__ __forceinline__ MaxSum max_sum(const T* chunks, int lo, int hi) {
     using R = Row<T>;
-    constexpr int E = R::E;
+    MaxSum v;
+    u32x4 q[kBatch];
+    int c = lo + threadIdx.x;
+    for (; c + (kBatch - 1) * TB < hi; c += kBatch * TB) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) q[k] = R::load(chunks + (c + k * TB) * R::E);
+        add_chunks<T, kBatch>(v, q);
+    }
+    for (; c < hi; c += TB) {
+        q[0] = R::load(chunks + c * R::E);
+        add_chunks<T, 1>(v, q);
+    }
+    return v;
+}
+__device__ __forceinline__ void add_value(MaxSum& v, float z) { v.add(z, z == -INFINITY ? 0.f : __expf(z - z)); }
+
+// The forward: rows of any length, read once.
+template <typename T, int TB>
+__global__ __launch_bounds__(TB) void lp_fwd_k(LpRows a) {
     __shared__ float red[2 * (TB / kWave)];
     const int64_t r = a.first + blockIdx.x;
     const int V = (int)a.V, tid = threadIdx.x;
     const int64_t y = a.targets[r];
     const T* row = static_cast<const T*>(a.logits) + r * a.V;
-    T* out = static_cast<T*>(a.grad) + r * a.V;
     float w;
-    if (!row_counts<T, OP>(a, r, y, w)) return;
-    const RowToken<OP> token(a, r);
+    if (!row_live<LpOp::FWD>(a, r, y, w, true)) return;
     const Span<T> sp(row, V);
-    const int h = sp.h, nb = sp.nb, ej = sp.edge(tid, V);
+    const int ej = sp.edge(tid, V);
     const float zy = to_f32<T>(row[y]), ez = ej >= 0 ? to_f32<T>(row[ej]) : -INFINITY;
-    const int whole = nb / (kBatch * TB) * (kBatch * TB);  // chunks in batches that every lane fills
-    MaxSum v;
-    u32x4 q[kBatch];
-    for (int c = tid; c < whole; c += kBatch * TB) {
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) q[k] = R::load(row + h + (c + k * TB) * E);
-        add_chunks<T, kBatch>(v, q);
-    }
-    for (int c = whole + tid; c < nb; c += TB) {
-        q[0] = R::load(row + h + c * E);
-        add_chunks<T, 1>(v, q);
-    }
-    v.add(ez, ez == -INFINITY ? 0.f : __expf(ez - ez));
+    MaxSum v = max_sum<T, TB>(row + sp.h, 0, sp.nb);
+    add_value(v, ez);
     v = block_max_sum(v, red);
-    if constexpr (OP == LpOp::FWD) {
-        if (tid == 0) a.logp[r] = (zy - v.m) - logf(v.s);
-        return;
-    }
-    // (all have read zy: from here the row may be overwritten)
-    const float logp = (zy - v.m) - logf(v.s);
-    const RowGrad<true> grad(RowExp<true>(v.m), a.cap, token.coef(a, w, logp), v.s, 0.f);
-    auto emit = [&](int c, u32x4 z) {
-        float x[E];
-#pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = h + c * E + i == y ? grad.target(zy) : grad(R::get(z, i));
-        R::store(out + h + c * E, R::pack(x));
-    };
-    for (int c = tid; c < whole; c += kBatch * TB) {
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) q[k] = R::load(row + h + (c + k * TB) * E);
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) emit(c + k * TB, q[k]);
-    }
-    for (int c = whole + tid; c < nb; c += TB) emit(c, R::load(row + h + c * E));
-    if (ej >= 0) out[ej] = from_f32<T>(ej == y ? grad.target(zy) : grad(ez));
-    if (tid == 0) token.finish(a, r, w, logp);
+    if (tid == 0) a.logp[r] = (zy - v.m) - logf(v.s);
 }
 
-// The same for rows of up to (NV + NL) TB chunks of 16 bytes, held on the CU, NV
-// a lane in registers and NL in LDS: one read, and the maximum before the
-// exponentials.  Only rows with a chunk may come to an instance with SURE > 0:
+// The gradient of rows of up to (NV + NL) TB chunks of 16 bytes, held on the
+// CU, NV a lane in registers and NL in LDS: one read, and the maximum before the
+// exponentials.  REST: longer rows, of which what is not held is read again for
+// the gradient, first, while it may be cached.  Only rows with a chunk may come to an instance with SURE > 0:
 // its first SURE steps ask no question (the row's last chunk is loaded where a
 // lane has none, and not used).
-template <typename T, LpOp OP, int TB, int NV, int SURE, int NL = 0>
+template <typename T, LpOp OP, int TB, int NV, int SURE, int NL = 0, bool REST = false>
 __global__ __launch_bounds__(TB, NV > 9 ? 4 : 8) void lp_held_k(LpRows a) {
     using R = Row<T>;
     constexpr int E = R::E, N = NV + NL;
@@ -323,7 +308,9 @@ __global__ __launch_bounds__(TB, NV > 9 ? 4 : 8) void lp_held_k(LpRows a) {
     const int ej = sp.edge(tid, V);
     float ez = ej >= 0 ? to_f32<T>(row[ej]) : -INFINITY;
     float zy = to_f32<T>(row[y]);
-    float mt = ez;
+    MaxSum rest;
+    if constexpr (REST) rest = max_sum<T, TB>(row + h, N * TB, nb);
+    float mt = fmaxf(ez, rest.m);
 #pragma unroll
     for (int k = 0; k < N; ++k)
         if (there(k)) {
@@ -350,11 +337,13 @@ __global__ __launch_bounds__(TB, NV > 9 ? 4 : 8) void lp_held_k(LpRows a) {
             }
         ez -= m;
         zy -= m;
+        rest.m -= m;
         z0 = m;
         m = 0.f;
     }
     const RowExp<false> ex(m);
     float st = ex(ez);
+    if constexpr (REST) st += rest.s * ex(rest.m);
 #pragma unroll
     for (int k = 0; k < N; ++k)
         if (there(k)) {
@@ -369,21 +358,31 @@ __global__ __launch_bounds__(TB, NV > 9 ? 4 : 8) void lp_held_k(LpRows a) {
     const float logp = ex.logp(zy, st);
     const RowGrad<false> grad(ex, a.cap, token.coef(a, w, logp), st, z0);
     const int yc = y < h ? -1 : ((int)y - h) / E, yi = y < h ? 0 : ((int)y - h) % E;
+    auto emit = [&](int c, u32x4 v, float less) {
+        float x[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = grad(R::get(v, i) - less);
+        if (c == yc) {
+            const float t = grad.target(zy);
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] = i == yi ? t : x[i];
+        }
+        R::store(out + h + c * E, R::pack(x));
+    };
+    if constexpr (REST) {
+        int c = N * TB + tid;
+        for (; c + (kBatch - 1) * TB < nb; c += kBatch * TB) {
+            u32x4 v[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) v[k] = R::load(row + h + (c + k * TB) * E);
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) emit(c + k * TB, v[k], z0);
+        }
+        for (; c < nb; c += TB) emit(c, R::load(row + h + c * E), z0);
+    }
 #pragma unroll
     for (int k = 0; k < N; ++k)
-        if (there(k)) {
-            const int c = tid + k * TB;
-            const u32x4 v = chunk(k);
-            float x[E];
-#pragma unroll
-            for (int i = 0; i < E; ++i) x[i] = grad(R::get(v, i));
-            if (c == yc) {
-                const float t = grad.target(zy);
-#pragma unroll
-                for (int i = 0; i < E; ++i) x[i] = i == yi ? t : x[i];
-            }
-            if (c < nb) R::store(out + h + c * E, R::pack(x));
-        }
+        if (there(k) && tid + k * TB < nb) emit(tid + k * TB, chunk(k), 0.f);
     if (ej >= 0) out[ej] = from_f32<T>(ej == y ? grad.target(zy) : grad(ez));
     if (tid == 0) token.finish(a, r, w, logp);
 }
@@ -402,7 +401,6 @@ constexpr int kSplitBlock = 256;
 
 template <typename T, LpOp OP>
 __global__ __launch_bounds__(kSplitBlock) void lp_part_k(LpRows a, Split sp) {
-    using R = Row<T>;
     __shared__ float red[2 * (kSplitBlock / kWave)];
     const int64_t r = blockIdx.y;
     const int V = (int)a.V, tid = threadIdx.x;
@@ -412,22 +410,8 @@ __global__ __launch_bounds__(kSplitBlock) void lp_part_k(LpRows a, Split sp) {
     const T* row = static_cast<const T*>(a.logits) + r * a.V;
     const Span<T> s(row, V);
     const int hi = sp.hi(s.nb), ej = blockIdx.x == 0 ? s.edge(tid, V) : -1;
-    MaxSum v;
-    u32x4 q[kBatch];
-    int c = sp.lo(s.nb) + tid;
-    for (; c + (kBatch - 1) * kSplitBlock < hi; c += kBatch * kSplitBlock) {
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) q[k] = R::load(row + s.h + (c + k * kSplitBlock) * R::E);
-        add_chunks<T, kBatch>(v, q);
-    }
-    for (; c < hi; c += kSplitBlock) {
-        q[0] = R::load(row + s.h + c * R::E);
-        add_chunks<T, 1>(v, q);
-    }
-    if (ej >= 0) {
-        const float ez = to_f32<T>(row[ej]);
-        v.add(ez, ez == -INFINITY ? 0.f : __expf(ez - ez));
-    }
+    MaxSum v = max_sum<T, kSplitBlock>(row + s.h, sp.lo(s.nb), hi);
+    if (ej >= 0) add_value(v, to_f32<T>(row[ej]));
     v = block_max_sum(v, red);
     if (tid == 0) {
         sp.part[r * sp.parts + blockIdx.x] = v;
@@ -483,12 +467,12 @@ __global__ __launch_bounds__(kSplitBlock) void lp_apply_k(LpRows a, Split sp) {
 
 // Splitting reads the row twice and takes two launches: for long rows of which
 // there are too few to fill the card.  Unsplit and split, us a call (7 to 9 of
-// them the host's): gradient of 1, 64, 128 rows of 131072 bf16 values 18.5 9.7,
-// 21.3 13.5, 25.2 20.8; of 1, 128 of 65536 fp32 10.8 9.7, 17.9 18.8; the forward
-// of 3 rows of 131072 bf16 10.9 9.3, of 1 of 65536 fp32 7.7 9.6.
+// them the host's): gradient of 1, 64, 128 rows of 131072 bf16 values 17.8 9.5,
+// 20.8 11.6, 24.4 19.1; of 65536 fp32 10.2 9.4, 12.8 9.9, 17.6 17.1; the forward
+// of 1, 128 rows of 150001 bf16 9.0 9.1, 11.0 11.0, of 300000 14.9 9.0, 17.9 16.9.
 constexpr int64_t kSplitRows = 128, kSplitValues = 65536, kPartChunks = 4 * kSplitBlock;
 int split_parts(LpOp op, int64_t n, int64_t V, int E) {
-    if (n > kSplitRows || V < kSplitValues + (op == LpOp::FWD)) return 1;
+    if (n > kSplitRows || V < (op == LpOp::FWD ? 3 * kSplitValues : kSplitValues)) return 1;
     int64_t p = cdiv(cdiv(V, E), kPartChunks);
     if (p > 1024 / n) p = 1024 / n;
     return (int)(p > kWave ? kWave : p);
@@ -517,7 +501,7 @@ void launch_grad(hipStream_t st, const LpRows& a, unsigned g) {
     else if (nc <= 1024 * 8) AR_HELD(1024, 8);
     else if (nc <= 1024 * (HR + 4)) lp_held_k<T, OP, 1024, HR, 8, 4><<<g, 1024, 0, st>>>(a);
     else if (nc <= 1024 * 16) AR_HELD(1024, 16);
-    else lp_row_k<T, OP, 1024><<<g, 1024, 0, st>>>(a);
+    else lp_held_k<T, OP, 1024, 16, 16, 0, true><<<g, 1024, 0, st>>>(a);
 #undef AR_HELD
 }
 
@@ -528,9 +512,9 @@ void launch_grad(hipStream_t st, const LpRows& a, unsigned g) {
 template <typename T>
 void launch_fwd(hipStream_t st, const LpRows& a, unsigned g) {
     const int64_t nc = cdiv(a.V, Row<T>::E);
-    if (nc <= 256) lp_row_k<T, LpOp::FWD, 64><<<g, 64, 0, st>>>(a);
-    else if (nc <= 2048 && a.n > 256) lp_row_k<T, LpOp::FWD, 256><<<g, 256, 0, st>>>(a);
-    else lp_row_k<T, LpOp::FWD, 1024><<<g, 1024, 0, st>>>(a);
+    if (nc <= 256) lp_fwd_k<T, 64><<<g, 64, 0, st>>>(a);
+    else if (nc <= 2048 && a.n > 256) lp_fwd_k<T, 256><<<g, 256, 0, st>>>(a);
+    else lp_fwd_k<T, 1024><<<g, 1024, 0, st>>>(a);
 }
 
 template <typename T, LpOp OP>
