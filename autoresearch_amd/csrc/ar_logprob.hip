@@ -292,16 +292,23 @@ __global__ __launch_bounds__(TB) void lp_fwd_k(LpRows a) {
 // The gradient of rows of up to (NV + NL) TB chunks of 16 bytes, held on the
 // CU, NV a lane in registers and NL in LDS: one read, and the maximum before the
 // exponentials.  REST: longer rows, of which what is not held is read again for
-// the gradient, first, while it may be cached.  Only rows with a chunk may come to an instance with SURE > 0:
-// its first SURE steps ask no question (the row's last chunk is loaded where a
-// lane has none, and not used).
+// the gradient, first, while it may be cached, past the caches of which the
+// gradient is written (1000 rows of 300001 fp32 values: 700 -> 640 us, and with
+// a pass that reads the gradient next 940 -> 842; shorter rows gain nothing, and
+// what reads 128 MB of gradient next takes 45 us for 21).
+// Rows go last to first: what the forward or the logits' product left in the
+// cache is read before it is gone, and what reads the gradient next finds its
+// first rows there (256 MB of fp32 and a pass over it 175 -> 160 us).
+// Only rows with a chunk may come to an instance with SURE > 0: its first SURE
+// steps ask no question (the row's last chunk is loaded where a lane has none,
+// and not used).
 template <typename T, LpOp OP, int TB, int NV, int SURE, int NL = 0, bool REST = false>
 __global__ __launch_bounds__(TB, NV > 9 ? 4 : 8) void lp_held_k(LpRows a) {
     using R = Row<T>;
     constexpr int E = R::E, N = NV + NL;
     __shared__ float red[2 * (TB / kWave)];
     __shared__ u32x4 more[NL ? NL * TB : 1];  // lane t's: t, t + TB, ...
-    const int64_t r = a.first + blockIdx.x;
+    const int64_t r = a.first + (gridDim.x - 1 - blockIdx.x);
     const int V = (int)a.V, tid = threadIdx.x;
     const int64_t y = a.targets[r];
     const T* row = static_cast<const T*>(a.logits) + r * a.V;
@@ -384,7 +391,8 @@ __global__ __launch_bounds__(TB, NV > 9 ? 4 : 8) void lp_held_k(LpRows a) {
 #pragma unroll
             for (int i = 0; i < E; ++i) x[i] = i == yi ? t : x[i];
         }
-        R::store(out + h + c * E, R::pack(x));
+        if constexpr (REST) R::store_nt(out + h + c * E, R::pack(x));
+        else R::store(out + h + c * E, R::pack(x));
     };
     if constexpr (REST) {
         int c = N * TB + tid;
