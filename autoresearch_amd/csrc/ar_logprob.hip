@@ -292,10 +292,9 @@ __global__ __launch_bounds__(TB) void lp_fwd_k(LpRows a) {
 // The gradient of rows of up to (NV + NL) TB chunks of 16 bytes, held on the
 // CU, NV a lane in registers and NL in LDS: one read, and the maximum before the
 // exponentials.  REST: longer rows, of which what is not held is read again for
-// the gradient, first, while it may be cached, past the caches of which the
-// gradient is written (1000 rows of 300001 fp32 values: 700 -> 640 us, and with
-// a pass that reads the gradient next 940 -> 842; shorter rows gain nothing, and
-// what reads 128 MB of gradient next takes 45 us for 21).
+// the gradient, which is written past the caches (1000 rows of 300001 fp32
+// values: 700 -> 640 us, and with a pass that reads the gradient next 940 -> 842;
+// shorter rows gain nothing, and a pass over 128 MB of gradient takes 45 us for 21).
 // Rows go last to first: what the forward or the logits' product left in the
 // cache is read before it is gone, and what reads the gradient next finds its
 // first rows there (256 MB of fp32 and a pass over it 175 -> 160 us).
@@ -306,6 +305,7 @@ template <typename T, LpOp OP, int TB, int NV, int SURE, int NL = 0, bool REST =
 __global__ __launch_bounds__(TB, NV > 9 ? 4 : 8) void lp_held_k(LpRows a) {
     using R = Row<T>;
     constexpr int E = R::E, N = NV + NL;
+    constexpr bool kFirst = NV > 9;  // registers for the rest's chunks beside those held
     __shared__ float red[2 * (TB / kWave)];
     __shared__ u32x4 more[NL ? NL * TB : 1];  // lane t's: t, t + TB, ...
     const int64_t r = a.first + (gridDim.x - 1 - blockIdx.x);
@@ -319,6 +319,11 @@ __global__ __launch_bounds__(TB, NV > 9 ? 4 : 8) void lp_held_k(LpRows a) {
     const Span<T> sp(row, V);
     const int h = sp.h, nb = sp.nb;
     const u32x4 none = R::fill(-INFINITY);
+    MaxSum rest;
+    if constexpr (REST && !kFirst) {
+        rest = max_sum<T, TB>(row + h, N * TB, nb);
+        __builtin_amdgcn_sched_barrier(0);
+    }
     u32x4 q[N];  // from NV on only until they are in LDS
     auto there = [&](int k) { return k < SURE || k * TB < nb; };
     auto chunk = [&](int k) { return k < NV ? q[k] : more[(k - NV) * TB + tid]; };
@@ -332,8 +337,7 @@ __global__ __launch_bounds__(TB, NV > 9 ? 4 : 8) void lp_held_k(LpRows a) {
     const int ej = sp.edge(tid, V);
     float ez = ej >= 0 ? to_f32<T>(row[ej]) : -INFINITY;
     float zy = to_f32<T>(row[y]);
-    MaxSum rest;
-    if constexpr (REST) rest = max_sum<T, TB>(row + h, N * TB, nb);
+    if constexpr (REST && kFirst) rest = max_sum<T, TB>(row + h, N * TB, nb);
     float mt = fmaxf(ez, rest.m);
 #pragma unroll
     for (int k = 0; k < N; ++k)
@@ -394,7 +398,7 @@ __global__ __launch_bounds__(TB, NV > 9 ? 4 : 8) void lp_held_k(LpRows a) {
         if constexpr (REST) R::store_nt(out + h + c * E, R::pack(x));
         else R::store(out + h + c * E, R::pack(x));
     };
-    if constexpr (REST) {
+    auto emit_rest = [&] {
         int c = N * TB + tid;
         for (; c + (kBatch - 1) * TB < nb; c += kBatch * TB) {
             u32x4 v[kBatch];
@@ -404,10 +408,15 @@ __global__ __launch_bounds__(TB, NV > 9 ? 4 : 8) void lp_held_k(LpRows a) {
             for (int k = 0; k < kBatch; ++k) emit(c + k * TB, v[k], z0);
         }
         for (; c < nb; c += TB) emit(c, R::load(row + h + c * E), z0);
-    }
+    };
+    if constexpr (REST && kFirst) emit_rest();
 #pragma unroll
     for (int k = 0; k < N; ++k)
         if (there(k) && tid + k * TB < nb) emit(tid + k * TB, chunk(k), 0.f);
+    if constexpr (REST && !kFirst) {
+        __builtin_amdgcn_sched_barrier(0);
+        emit_rest();
+    }
     if (ej >= 0) out[ej] = from_f32<T>(ej == y ? grad.target(zy) : grad(ez));
     if (tid == 0) token.finish(a, r, w, logp);
 }
@@ -510,8 +519,11 @@ int split_parts(LpOp op, int64_t n, int64_t V, int E) {
 // per chunk and takes four: 8192 values 256 x 4 5.8, 512 x 2 5.6, 1024 x 1 3.7.
 // Two workgroups of 1024 fit a CU with up to 64 registers and 80 KiB of LDS
 // each, one with more, whose reads, sums and writes then take turns: 90000 bf16
-// values 8 chunks in registers and 4 in LDS 5.0, 16 in registers 4.6; 131072
-// 4.8 (bound by arithmetic: fp32 rows of those bytes 5.3); 50001 fp32 5.0, 4.7.
+// values 8 chunks in registers and 4 in LDS 5.0, 16 in registers 4.6; 50001 fp32
+// 5.0, 4.7.  Two with a part of the row read again or one, which reads less of it
+// again and has the cache to itself: 131072 bf16 4.7 4.0, 150001 4.5 4.2, 180000
+// 4.5 4.5, 256000 4.5 4.6; 65536 fp32 5.1 5.1, 80001 4.7 4.8, 300001 3.4 4.2.  (One
+// that keeps 8 more chunks in LDS: 256000 bf16 4.6, 300001 fp32 4.1.)
 template <typename T, LpOp OP>
 void launch_grad(hipStream_t st, const LpRows& a, unsigned g) {
     const int64_t nc = cdiv(a.V, Row<T>::E);
@@ -525,7 +537,7 @@ void launch_grad(hipStream_t st, const LpRows& a, unsigned g) {
     else if (nc <= 1024 * 4) AR_HELD(1024, 4);
     else if (nc <= 1024 * 8) AR_HELD(1024, 8);
     else if (nc <= 1024 * (HR + 4)) lp_held_k<T, OP, 1024, HR, 8, 4><<<g, 1024, 0, st>>>(a);
-    else if (nc <= 1024 * 16) AR_HELD(1024, 16);
+    else if (nc <= 1024 * 20) lp_held_k<T, OP, 1024, 8, 8, 4, true><<<g, 1024, 0, st>>>(a);
     else lp_held_k<T, OP, 1024, 16, 16, 0, true><<<g, 1024, 0, st>>>(a);
 #undef AR_HELD
 }
