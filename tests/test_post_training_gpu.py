@@ -152,7 +152,8 @@ def test_gradient_of_other_alignment_than_logits(env):
         n, V = 5, 4099
         z, y, _ = make_logits(torch, n, V, dt, 4, 15.0, off=2)
         g = torch.randn(n, device="cuda")
-        a, b = torch.empty(n, V, dtype=dt, device="cuda"), torch.empty(n * V + 3, dtype=dt, device="cuda")[3:].view(n, V)
+        a = torch.empty(n, V, dtype=dt, device="cuda")
+        b = torch.empty(n * V + 3, dtype=dt, device="cuda")[3:].view(n, V)
         ops.token_logprob_bwd(a, z, y, g, 15.0, n, V)
         ops.token_logprob_bwd(b, z, y, g, 15.0, n, V)
         assert torch.equal(a, b)
@@ -162,10 +163,19 @@ def test_gradient_of_other_alignment_than_logits(env):
 @pytest.mark.parametrize("V", [5, 513, 8192, 40001, 131079])
 @pytest.mark.parametrize("n", [8, 700])
 def test_rows_of_infinities_and_nan(env, V, dtype, n):
+    check_rows_of_infinities_and_nan(env, V, dtype, min(n, 10_000_000 // V))
+
+
+# rows too many to be split over workgroups, of which a part is read again
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("V", [70001, 131079, 270001])
+def test_many_long_rows_of_infinities_and_nan(env, V, dtype):
+    check_rows_of_infinities_and_nan(env, V, dtype, 130)
+
+
+def check_rows_of_infinities_and_nan(env, V, dtype, n):
     torch, ops = env
     dt = getattr(torch, dtype)
-    if n * V > 10_000_000:
-        n = 10_000_000 // V
     z, y, _ = make_logits(torch, n, V, dt, V, 0.0)
     y[:8] = torch.tensor([V - 1, 0, 0, 0, -1, V + 5, 1, 1], device="cuda")
     z[0, : V - 1] = -math.inf          # one value left
@@ -194,14 +204,25 @@ def test_rows_of_infinities_and_nan(env, V, dtype, n):
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("V", [9, 513, 8192, 40001, 150001, 270001])
 def test_rows_of_far_values(env, V, dtype):
+    check_rows_of_far_values(env, V, dtype, 1)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("V", [70001, 131079, 270001])
+def test_many_long_rows_of_far_values(env, V, dtype):
+    check_rows_of_far_values(env, V, dtype, 12)
+
+
+def check_rows_of_far_values(env, V, dtype, times):
     """Rows whose largest value is far from zero, on both sides of 2^20, or the type's lowest or largest value."""
     torch, ops = env
     dt = getattr(torch, dtype)
-    top = [1048575.0, 1048576.0, 1.0e6, 3.0e6, -1.0e6, -3.0e6, 1e9, -1e9, 3e37, torch.finfo(dt).min, torch.finfo(dt).max]
+    lowest, largest = torch.finfo(dt).min, torch.finfo(dt).max
+    top = [1048575.0, 1048576.0, 1.0e6, 3.0e6, -1.0e6, -3.0e6, 1e9, -1e9, 3e37, lowest, largest] * times
     n = len(top)
     g = gen(torch, V)
     z = (torch.tensor(top, device="cuda", dtype=torch.float64)[:, None]
-         - torch.rand(n, V, generator=g, device="cuda").double() * 4).clamp(torch.finfo(dt).min, torch.finfo(dt).max).to(dt)
+         - torch.rand(n, V, generator=g, device="cuda").double() * 4).clamp(lowest, largest).to(dt)
     z[:, 0] = torch.tensor(top, device="cuda", dtype=torch.float64).to(dt)
     y = torch.randint(0, V, (n,), generator=g, device="cuda")
     z[2, 1:] = 0.0  # one value holds all
@@ -364,12 +385,23 @@ def test_descending_and_outside_offsets_stay_inside(env):
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("V", [9, 512, 2050, 8192, 32768, 40001, 131079])
-@pytest.mark.parametrize("n,start,per_seq", [(40, [0, 11, 11, 38], True), (3, [0, 3], False), (601, [1, 300, 600], True)])
+@pytest.mark.parametrize("n,start,per_seq",
+                         [(40, [0, 11, 11, 38], True), (3, [0, 3], False), (601, [1, 300, 600], True)])
 def test_policy_loss_from_logits(env, V, dtype, n, start, per_seq):
-    torch, ops = env
-    dt = getattr(torch, dtype)
     if n * V > 12_000_000:
         n, start = 80, [0, 3, 79]
+    check_policy_loss_from_logits(env, V, dtype, n, start, per_seq)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("V", [50001, 70001, 90002, 131079, 270001])
+def test_policy_loss_from_many_long_rows(env, V, dtype):
+    check_policy_loss_from_logits(env, V, dtype, 131, [0, 70, 130], True)
+
+
+def check_policy_loss_from_logits(env, V, dtype, n, start, per_seq):
+    torch, ops = env
+    dt = getattr(torch, dtype)
     cap = 15.0 if V % 2 == 0 else 0.0
     z, y, _ = make_logits(torch, n, V, dt, V + n, cap)
     y[1], y[2] = (-1, V) if n > 3 else (y[1], y[2])
@@ -463,7 +495,7 @@ def test_preference_loss(env, n, start, smooth, with_ref):
     args = (logp, ref, y, st, beta, smooth, n, P, V)
     ops.preference_loss(loss, margin, grad, *args, 3.0)
     _, ok, seq, cnt = ref_weights(torch, y, st, V, False)
-    diff = torch.where(ok, logp.double() - (ref.double() if with_ref else 0.0), torch.zeros(n, dtype=torch.float64, device="cuda"))
+    diff = torch.where(ok, logp.double() - (ref.double() if with_ref else 0.0), 0.0)
     sums = torch.zeros(2 * P, dtype=torch.float64, device="cuda").index_add_(0, seq.clamp(min=0), diff)
     cnt = torch.tensor(cnt, device="cuda")
     live = (cnt[0::2] > 0) & (cnt[1::2] > 0)
@@ -471,7 +503,7 @@ def test_preference_loss(env, n, start, smooth, with_ref):
     sp = torch.nn.functional.softplus
     pairs = max(1, int(live.sum()))
     lp = torch.where(live, (1 - smooth) * sp(-h) + smooth * sp(h), torch.zeros_like(h))
-    slope = torch.where(live, beta * (smooth * torch.sigmoid(h) - (1 - smooth) * torch.sigmoid(-h)) / pairs, torch.zeros_like(h))
+    slope = torch.where(live, beta * (smooth * torch.sigmoid(h) - (1 - smooth) * torch.sigmoid(-h)) / pairs, 0.0)
     sign = torch.stack([slope, -slope], 1).reshape(-1)
     G = torch.where(ok, sign[seq.clamp(min=0)], torch.zeros_like(diff))
     close(torch, loss[:1], lp.sum()[None] / pairs, 2.0 ** -40, torch.float32)
@@ -522,7 +554,8 @@ def test_clip_grad_norm(env, sizes, dtype, factor, off):
     c = min(1.0, factor)
     for x, o in zip(grads, outs):
         # product and quotient in fp64, a rounding to fp32 on the way to bf16
-        close(torch, o, x.double() * c, (2 * U if x.dtype == torch.bfloat16 else n * 2.0 ** -52) * x.double().abs(), x.dtype)
+        rel = 2 * U if x.dtype == torch.bfloat16 else n * 2.0 ** -52
+        close(torch, o, x.double() * c, rel * x.double().abs(), x.dtype)
         if c == 1.0:
             assert torch.equal(o, x)
     inplace = [x.clone() for x in grads]
