@@ -122,7 +122,7 @@ __device__ __forceinline__ MaxSum block_max_sum(MaxSum v, float* red) {
 // row waits for coef, its gradient by logp (w: the token's weight or
 // gradient); what else the token has comes behind the row's last store, in one
 // lane (65536 rows of 8192 fp32 values: both before the row in fp64 798 us, in
-// fp32 725, so 713).
+// fp32 725, so 704).
 template <LpOp OP>
 struct RowToken {
     __device__ __forceinline__ RowToken(const LpRows&, int64_t) {}
@@ -143,11 +143,27 @@ struct RowToken<LpOp::POLICY> {
     }
 };
 
+// log2 of a sum: its exponent, and the logarithm of its mantissa (in
+// [sqrt(1/2), sqrt(2)): off by 2^-25).  Sums over tokens add up what
+// log-probabilities are off by, so they are put together in fp64 and rounded
+// once (the forward of 131072 rows of 1024 bf16 values: 51 us; with all of the
+// logarithm in fp64, 64).
+__device__ __forceinline__ double log2_sum(float s) {
+    float f = __builtin_amdgcn_frexp_mantf(s);
+    int e = __builtin_amdgcn_frexp_expf(s);
+    if (f < 0.707106781f) {
+        f *= 2.f;
+        --e;
+    }
+    return (double)e + (double)log2f(f);
+}
+constexpr double kLn2 = 0.6931471805599453;
+
 // exp(z - m).  SUB: the difference first.  Otherwise one fma and the hardware's
 // exponential: z log2 e - m log2 e, rounded once.  The second product's own
 // rounding is a factor common to the whole row, which the sum has too; it is
 // small up to |m| = 2^20, and the caller sees to that.
-constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+constexpr float kLog2e = 1.44269504f;
 constexpr float kFar = 1048576.f;
 template <bool SUB>
 struct RowExp {
@@ -160,7 +176,7 @@ struct RowExp {
     // log-probability of z where the row's exponentials sum up to s
     __device__ __forceinline__ float logp(float z, float s) const {
         const float common = SUB ? 0.f : fmaf(m, kLog2e, c);  // log2 of the row's common factor
-        return (z - m) - fmaf(log2f(s), kLn2, -common * kLn2);
+        return (float)((double)z - (double)m - (log2_sum(s) - (double)common) * kLn2);
     }
 };
 
@@ -256,20 +272,6 @@ __device__ __forceinline__ MaxSum max_sum(const T* chunks, int lo, int hi) {
 }
 __device__ __forceinline__ void add_value(MaxSum& v, float z) { v.add(z, z == -INFINITY ? 0.f : __expf(z - z)); }
 
-// The log-probability, rounded once but for the logarithm of the sum's mantissa
-// (in [sqrt(1/2), sqrt(2)): off by 2^-25): sums over tokens add up what it is
-// off by.  131072 rows of 1024 bf16 values: 51 us; with the whole logarithm in
-// fp64, 64.
-__device__ __forceinline__ float row_logp(float zy, MaxSum v) {
-    float f = __builtin_amdgcn_frexp_mantf(v.s);
-    int e = __builtin_amdgcn_frexp_expf(v.s);
-    if (f < 0.707106781f) {
-        f *= 2.f;
-        --e;
-    }
-    return (float)((double)zy - (double)v.m - ((double)e + (double)log2f(f)) * 0.6931471805599453);
-}
-
 // The forward: rows of any length, read once.
 template <typename T, int TB>
 __global__ __launch_bounds__(TB) void lp_fwd_k(LpRows a) {
@@ -286,7 +288,7 @@ __global__ __launch_bounds__(TB) void lp_fwd_k(LpRows a) {
     MaxSum v = max_sum<T, TB>(row + sp.h, 0, sp.nb);
     add_value(v, ez);
     v = block_max_sum(v, red);
-    if (tid == 0) a.logp[r] = row_logp(zy, v);
+    if (tid == 0) a.logp[r] = RowExp<true>(v.m).logp(zy, v.s);
 }
 
 // The gradient of rows of up to (NV + NL) TB chunks of 16 bytes, held on the
@@ -464,7 +466,7 @@ __global__ __launch_bounds__(kWave) void lp_join_k(LpRows a, Split sp) {
     float w;
     if (!row_live<LpOp::FWD>(a, r, a.targets[r], w, true)) return;
     const MaxSum v = join_parts(sp, r);
-    if (threadIdx.x == 0) a.logp[r] = row_logp(sp.zy[r], v);
+    if (threadIdx.x == 0) a.logp[r] = RowExp<true>(v.m).logp(sp.zy[r], v.s);
 }
 template <typename T, LpOp OP>
 __global__ __launch_bounds__(kSplitBlock) void lp_apply_k(LpRows a, Split sp) {
@@ -486,8 +488,9 @@ __global__ __launch_bounds__(kSplitBlock) void lp_apply_k(LpRows a, Split sp) {
     const RowToken<OP> token(a, r);
     const MaxSum v = join_parts(sp, r);
     const float zy = sp.zy[r];
-    const float logp = (zy - v.m) - logf(v.s);
-    const RowGrad<true> grad(RowExp<true>(v.m), a.cap, token.coef(a, w, logp), v.s, 0.f);
+    const RowExp<true> ex(v.m);
+    const float logp = ex.logp(zy, v.s);
+    const RowGrad<true> grad(ex, a.cap, token.coef(a, w, logp), v.s, 0.f);
     for (int c = sp.lo(s.nb) + tid; c < hi; c += kSplitBlock) {
         const u32x4 z = R::load(row + s.h + c * E);
         float x[E];
