@@ -129,6 +129,7 @@ __device__ __forceinline__ MaxSum block_max_sum(MaxSum v, float* red) {
 // fp32 725, so 704).
 template <LpOp OP>
 struct RowToken {
+    __device__ __forceinline__ explicit RowToken(const PolicyToken&) {}
     __device__ __forceinline__ RowToken(const LpRows&, int64_t) {}
     __device__ __forceinline__ float coef(const LpRows&, float w, float) const { return w; }
     __device__ __forceinline__ void finish(const LpRows&, int64_t, float, float) const {}
@@ -136,6 +137,7 @@ struct RowToken {
 template <>
 struct RowToken<LpOp::POLICY> {
     PolicyToken t;
+    __device__ __forceinline__ explicit RowToken(const PolicyToken& token) : t(token) {}
     __device__ __forceinline__ RowToken(const LpRows& a, int64_t r) : t(a.policy, r) {}
     __device__ __forceinline__ float coef(const LpRows& a, float w, float logp) const {
         return w * policy_slope(logp, t, a.policy) * a.loss_scale;
@@ -429,9 +431,11 @@ __global__ __launch_bounds__(TB, NV > 9 ? 4 : 8) void lp_held_k(LpRows a) {
 
 // ---- few long rows: each split over several workgroups ----
 // part[r][p]: the maximum and sum of part p's chunks, part 0 with the values
-// outside the chunks; zy[r]: the target's.
+// outside the chunks; zy[r]: the target's; token[r]: POLICY's inputs, of which
+// logp_out may be one (a row's workgroups end in any order).
 struct Split {
     MaxSum* part;
+    PolicyToken* token;
     float* zy;
     int parts;
     __device__ __forceinline__ int lo(int nb) const { return min(nb, (int)blockIdx.x * ((nb + parts - 1) / parts)); }
@@ -456,6 +460,7 @@ __global__ __launch_bounds__(kSplitBlock) void lp_part_k(LpRows a, Split sp) {
     if (tid == 0) {
         sp.part[r * sp.parts + blockIdx.x] = v;
         if (blockIdx.x == 0) sp.zy[r] = to_f32<T>(row[y]);
+        if (OP == LpOp::POLICY && blockIdx.x == 0) sp.token[r] = PolicyToken(a.policy, r);
     }
 }
 // The whole row's, by every wave.
@@ -489,7 +494,7 @@ __global__ __launch_bounds__(kSplitBlock) void lp_apply_k(LpRows a, Split sp) {
         if (ej >= 0) out[ej] = from_f32<T>(0.f);
         return;
     }
-    const RowToken<OP> token(a, r);
+    const RowToken<OP> token(OP == LpOp::POLICY ? sp.token[r] : PolicyToken());
     const MaxSum v = join_parts(sp, r);
     const float zy = sp.zy[r];
     const RowExp<true> ex(v.m);
@@ -564,7 +569,8 @@ void launch_fwd(hipStream_t st, const LpRows& a, unsigned g) {
 template <typename T, LpOp OP>
 void launch_split(hipStream_t st, const LpRows& a, int parts) {
     MaxSum* const part = static_cast<MaxSum*>(a.scratch);
-    const Split sp{part, reinterpret_cast<float*>(part + a.n * parts), parts};
+    PolicyToken* const token = reinterpret_cast<PolicyToken*>(part + a.n * parts);
+    const Split sp{part, token, reinterpret_cast<float*>(token + (OP == LpOp::POLICY ? a.n : 0)), parts};
     const dim3 g(parts, (unsigned)a.n);
     lp_part_k<T, OP><<<g, kSplitBlock, 0, st>>>(a, sp);
     if constexpr (OP == LpOp::FWD) lp_join_k<<<(unsigned)a.n, kWave, 0, st>>>(a, sp);
@@ -589,7 +595,7 @@ void launch(hipStream_t st, const LpRows& a) {
 
 size_t lp_scratch(LpOp op, bool bf16_logits, int64_t n, int64_t V) {
     const int parts = n > 0 ? split_parts(op, n, V, bf16_logits ? Row<bf16>::E : Row<float>::E) : 1;
-    return parts > 1 ? n * (parts * sizeof(MaxSum) + sizeof(float)) : 0;
+    return parts > 1 ? n * (parts * sizeof(MaxSum) + (op == LpOp::POLICY ? sizeof(PolicyToken) : 0) + sizeof(float)) : 0;
 }
 
 int32_t lp_rows(hipStream_t st, LpOp op, bool bf16_logits, const LpRows& a, const char* nm) {
@@ -601,7 +607,7 @@ int32_t lp_rows(hipStream_t st, LpOp op, bool bf16_logits, const LpRows& a, cons
 }
 
 int32_t check_rows(const char* nm, const void* logits, int32_t logits_bf16, const void* grad, const int64_t* targets,
-                   int64_t n, int64_t V) {
+                   const float* logp, int64_t n, int64_t V) {
     AR_CHECK_ARG(n >= 0 && V > 0, "%s: bad shape", nm);
     AR_CHECK_ARG(n == 0 || (logits && targets), "%s: null pointer", nm);
     AR_CHECK_ARG(logits_bf16 == 0 || logits_bf16 == 1, "%s: logits_bf16 must be 0 or 1", nm);
@@ -612,6 +618,8 @@ int32_t check_rows(const char* nm, const void* logits, int32_t logits_bf16, cons
                  "%s: logits or their gradient not aligned to a value", nm);
     AR_CHECK_ARG(grad == logits || !overlaps(grad, bytes, logits, bytes),
                  "%s: the gradient overlaps the logits without being them", nm);
+    AR_CHECK_ARG(!overlaps(logp, n * sizeof(float), logits, bytes) && !overlaps(logp, n * sizeof(float), grad, bytes),
+                 "%s: an array by token overlaps the logits or their gradient", nm);
     return AR_OK;
 }
 
@@ -632,7 +640,7 @@ extern "C" int32_t ar_token_logprob_fwd(ar_stream_t stream, float* logp_out, con
                                         const int64_t* targets, int64_t num_tokens, int64_t vocab_size) {
     AR_CHECK_ARG(num_tokens <= 0 || logp_out, "token_logprob_fwd: null pointer");
     if (const int32_t r =
-            check_rows("token_logprob_fwd", logits, logits_bf16, nullptr, targets, num_tokens, vocab_size))
+            check_rows("token_logprob_fwd", logits, logits_bf16, nullptr, targets, logp_out, num_tokens, vocab_size))
         return r;
     LpRows a;
     a.logits = logits;
@@ -648,8 +656,8 @@ extern "C" int32_t ar_token_logprob_bwd(ar_stream_t stream, void* grad_logits, c
                                         int64_t vocab_size) {
     AR_CHECK_ARG(num_tokens <= 0 || (grad_logits && grad_logp), "token_logprob_bwd: null pointer");
     AR_CHECK_ARG(cap >= 0.f, "token_logprob_bwd: cap must not be negative");
-    if (const int32_t r =
-            check_rows("token_logprob_bwd", logits, logits_bf16, grad_logits, targets, num_tokens, vocab_size))
+    if (const int32_t r = check_rows("token_logprob_bwd", logits, logits_bf16, grad_logits, targets, grad_logp,
+                                     num_tokens, vocab_size))
         return r;
     LpRows a;
     a.logits = logits;

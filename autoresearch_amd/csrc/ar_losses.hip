@@ -596,7 +596,9 @@ extern "C" int32_t ar_policy_loss_logits(ar_stream_t stream, float* loss_out, fl
     const char* nm = "policy_loss_logits";
     AR_CHECK_ARG(loss_out && (num_tokens <= 0 || grad_logits), "%s: null pointer", nm);
     AR_CHECK_ARG(cap >= 0.f, "%s: cap must not be negative", nm);
-    if (const int32_t r = check_rows(nm, logits, logits_bf16, grad_logits, targets, num_tokens, vocab_size)) return r;
+    if (const int32_t r =
+            check_rows(nm, logits, logits_bf16, grad_logits, targets, logp_out, num_tokens, vocab_size))
+        return r;
     if (const int32_t r = check_seqs(nm, targets, seq_start, num_tokens, num_seqs, vocab_size)) return r;
     if (const int32_t r = check_policy(nm, logp_out, nullptr, old_logp, ref_logp, advantages, num_tokens, clip_low,
                                        clip_high, kl_coef))

@@ -147,9 +147,10 @@ struct LpRows {
 };
 size_t lp_scratch(LpOp op, bool bf16_logits, int64_t n, int64_t V);
 int32_t lp_rows(hipStream_t st, LpOp op, bool bf16_logits, const LpRows& a, const char* nm);
-// What the entry points on logits check alike.
+// What the entry points on logits check alike; logp: an array by token that
+// the call reads for one row, or writes, while it works on others.
 int32_t check_rows(const char* nm, const void* logits, int32_t logits_bf16, const void* grad, const int64_t* targets,
-                   int64_t n, int64_t V);
+                   const float* logp, int64_t n, int64_t V);
 
 inline bool overlaps(const void* a, size_t na, const void* b, size_t nb) {
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);

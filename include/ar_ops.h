@@ -321,7 +321,7 @@ int32_t ar_policy_loss(ar_stream_t stream, float* loss_out, float* grad_logp, co
                        int64_t num_tokens, int64_t num_seqs, int64_t vocab_size, float loss_scale);
 /* The same from the logits, with its gradient by them, in one pass over the
  * logits: ar_token_logprob_fwd, ar_policy_loss and ar_token_logprob_bwd.
- * grad_logits may be logits; logp_out may be NULL. */
+ * grad_logits may be logits; logp_out may be NULL, or an input by token. */
 int32_t ar_policy_loss_logits(ar_stream_t stream, float* loss_out, float* logp_out, void* grad_logits,
                               const void* logits, int32_t logits_bf16, const float* old_logp, const float* ref_logp,
                               const float* advantages, const int64_t* targets, const int64_t* seq_start, float cap,

@@ -87,10 +87,18 @@ def test_rows_of_logits(lib, call, kw, code, word):
 @pytest.mark.parametrize("call", [bwd, policy_logits])
 @pytest.mark.parametrize("kw,word", [
     ({"grad": None}, "null"), ({"cap": -1.0}, "cap"), ({"cap": math.nan}, "cap"),
-    ({"grad": A["logits"] + 4}, "overlaps"), ({"grad": A["logits"] - 64}, "overlaps"), ({"grad": A["grad"] + 2}, "aligned"),
+    ({"grad": A["logits"] + 4}, "overlaps"), ({"grad": A["logits"] - 64}, "overlaps"),
+    ({"grad": A["grad"] + 2}, "aligned"),
 ])
 def test_gradient_of_logits(lib, call, kw, word):
     refused(lib, call(lib, **kw), EINVAL, word)
+
+
+@pytest.mark.parametrize("call", ROWS)
+def test_arrays_by_token_over_the_logits(lib, call):
+    refused(lib, call(lib, logp=A["logits"] + 8), EINVAL, "overlaps")
+    if call is not fwd:
+        refused(lib, call(lib, logp=A["grad"] + 100), EINVAL, "overlaps")
 
 
 def test_null_log_probabilities(lib):

@@ -443,6 +443,29 @@ def check_policy_loss_from_logits(env, V, dtype, n, start, per_seq):
     assert torch.equal(again, loss) and torch.equal(z2, out)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n,V", [(40, 131079), (128, 65537), (131, 65537), (300, 513), (9000, 64)])
+def test_log_probabilities_over_an_input(env, dtype, n, V):
+    """logp_out may be an input by token, also where a row is split over workgroups: the same bits."""
+    torch, ops = env
+    z, y, _ = make_logits(torch, n, V, getattr(torch, dtype), 3, 15.0)
+    g = gen(torch, 5)
+    old, ref, adv = (torch.randn(n, generator=g, device="cuda") for _ in range(3))
+    old, ref = old * 0.3 - math.log(V), ref * 0.3 - math.log(V)
+    st = torch.tensor([0, n // 3, n - 1], device="cuda")
+
+    def call(over):
+        ins = [old.clone(), ref.clone(), adv.clone()]
+        loss, out = torch.empty(2, device="cuda"), torch.empty_like(z)
+        logp = torch.empty(n, device="cuda") if over is None else ins[over]
+        ops.policy_loss_logits(loss, logp, out, z, *ins, y, st, 15.0, 0.2, 0.2, 0.1, True, n, 2, V)
+        return loss, logp, out
+
+    want = call(None)
+    for over in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(want, call(over))), over
+
+
 def test_policy_gradient_against_differences(env):
     """<gradient, v> against the loss's central difference along v, both losses in 64 bits."""
     torch, ops = env
