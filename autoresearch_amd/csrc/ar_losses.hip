@@ -282,16 +282,18 @@ __global__ __launch_bounds__(kSmallBlock) void policy_small_k(Seqs q, PolicyToke
     }
 }
 
-// The sums of a block's kSumPairs of part's n pairs, in a fixed order: to out
-// (n <= kSumPairs), or to part2 for another such launch.  One block for all of
-// 65536 pairs took 36 us, with eight loads in flight 23, in two launches 11.
-constexpr int64_t kSumPairs = 4096;
+// The sums of a block's PAIRS of part's n pairs, in a fixed order: to out (one
+// block), or to part2 for another such launch.  One block for all of 65536
+// pairs took 36 us, with eight loads in flight 23, in two launches 11; up to
+// kSumLast pairs one block is faster (8192: by 2.7 us, 16384: 1.5).
+constexpr int64_t kSumPairs = 4096, kSumLast = 16384;
+template <int64_t PAIRS>
 __global__ __launch_bounds__(1024) void sum_pairs_k(const double2* part, int64_t n, double2* part2, float* out) {
     __shared__ double red[16];
     double a = 0.0, b = 0.0;
 #pragma unroll
-    for (int k = 0; k < kSumPairs / 1024; ++k) {
-        const int64_t i = blockIdx.x * kSumPairs + threadIdx.x + k * 1024;
+    for (int k = 0; k < PAIRS / 1024; ++k) {
+        const int64_t i = blockIdx.x * PAIRS + threadIdx.x + k * 1024;
         const double2 v = i < n ? part[i] : make_double2(0.0, 0.0);
         a += v.x;
         b += v.y;
@@ -311,13 +313,14 @@ __global__ __launch_bounds__(1024) void sum_pairs_k(const double2* part, int64_t
 // How many pairs sum_pairs needs, for the sums of sums behind the n.
 int64_t pair_room(int64_t n) {
     int64_t room = n;
-    while (n > kSumPairs) room += n = cdiv(n, kSumPairs);
+    while (n > kSumLast) room += n = cdiv(n, kSumPairs);
     return room;
 }
 void sum_pairs(hipStream_t st, double2* part, int64_t n, float* out) {
-    for (; n > kSumPairs; part += n, n = cdiv(n, kSumPairs))
-        sum_pairs_k<<<(unsigned)cdiv(n, kSumPairs), 1024, 0, st>>>(part, n, part + n, nullptr);
-    sum_pairs_k<<<1, 1024, 0, st>>>(part, n, nullptr, out);
+    for (; n > kSumLast; part += n, n = cdiv(n, kSumPairs))
+        sum_pairs_k<kSumPairs><<<(unsigned)cdiv(n, kSumPairs), 1024, 0, st>>>(part, n, part + n, nullptr);
+    if (n > kSumPairs) sum_pairs_k<kSumLast><<<1, 1024, 0, st>>>(part, n, nullptr, out);
+    else sum_pairs_k<kSumPairs><<<1, 1024, 0, st>>>(part, n, nullptr, out);
 }
 
 // ---- preference ----

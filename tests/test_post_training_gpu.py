@@ -399,6 +399,12 @@ def test_policy_loss_from_many_long_rows(env, V, dtype):
     check_policy_loss_from_logits(env, V, dtype, 131, [0, 70, 130], True)
 
 
+# the losses of so many tokens are added up in one launch and in two
+@pytest.mark.parametrize("n", [2049, 4097, 16384, 16385, 70001])
+def test_policy_loss_from_many_rows(env, n):
+    check_policy_loss_from_logits(env, 9, "float32", n, [0, n // 3, n // 2, n - 7], n % 2 == 0)
+
+
 def check_policy_loss_from_logits(env, V, dtype, n, start, per_seq):
     torch, ops = env
     dt = getattr(torch, dtype)
