@@ -104,9 +104,10 @@ __global__ __launch_bounds__(1024) void totals_k(Seqs q, const int* cnt, Totals*
 }
 
 // What a token's term weighs: 1 / (all tokens that count), or 1 / (sequences
-// with one x this sequence's), rounded once to fp32.  Ahead of the sequences'
-// items every block takes the totals: from the counts where they are few, or
-// as totals_k left them.
+// with one x this sequence's); rounded to fp32 only on its way to rows of
+// logits, whose gradients are rounded again.  Ahead of the sequences' items
+// every block takes the totals: from the counts where they are few, or as
+// totals_k left them.
 struct Weights {
     Totals t;
     __device__ __forceinline__ Weights(const Seqs& q, const int* cnt, const Totals* total, TotalsLds& l) {
@@ -114,8 +115,8 @@ struct Weights {
         else t = sum_counts(q, cnt, l);
     }
     // of a token of an item, by every thread of the block
-    __device__ __forceinline__ float of(const Seqs& q, const int* cnt, int64_t item, int per_seq, int64_t* red) const {
-        if (!per_seq) return t.n ? (float)(1.0 / (double)t.n) : 0.f;
+    __device__ __forceinline__ double of(const Seqs& q, const int* cnt, int64_t item, int per_seq, int64_t* red) const {
+        if (!per_seq) return t.n ? 1.0 / (double)t.n : 0.0;
         const int64_t first = (int64_t)item_seq(q, item) * q.parts;
         int64_t ns = 0;
         if (q.parts == 1) {
@@ -124,7 +125,7 @@ struct Weights {
             for (int p = threadIdx.x; p < q.parts; p += blockDim.x) ns += cnt[first + p];
             ns = block_total(ns, red);
         }
-        return ns ? (float)(1.0 / ((double)t.alive * (double)ns)) : 0.f;
+        return ns ? 1.0 / ((double)t.alive * (double)ns) : 0.0;
     }
 };
 __global__ __launch_bounds__(kTokBlock) void weight_k(Seqs q, const int* cnt, const Totals* total, int per_seq,
@@ -135,7 +136,7 @@ __global__ __launch_bounds__(kTokBlock) void weight_k(Seqs q, const int* cnt, co
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
         int64_t lo, hi;
         item_range(q, item, lo, hi);
-        const float ws = w.of(q, cnt, item, per_seq, l.red);
+        const float ws = (float)w.of(q, cnt, item, per_seq, l.red);
         for (int64_t t = lo + threadIdx.x; t < hi; t += kTokBlock) weight[t] = counts(q, t) ? ws : 0.f;
     }
     each_outside(q, [&](int64_t t) { weight[t] = 0.f; });
@@ -156,9 +157,9 @@ struct Token {
     __device__ __forceinline__ Token() {}
     __device__ __forceinline__ Token(const Seqs& q, const PolicyTokens& a, int64_t t)
         : in(a.in, t), logp(a.logp[t]), live(counts(q, t)) {}
-    __device__ __forceinline__ void use(const PolicyTokens& a, int64_t t, float w, double& loss, double& kl) const {
+    __device__ __forceinline__ void use(const PolicyTokens& a, int64_t t, double w, double& loss, double& kl) const {
         float g = 0.f;
-        if (live && w != 0.f) {
+        if (live && w != 0.0) {
             const PolicyTerm<double> o = policy_term<double>(logp, in, a.in);
             loss += w * o.loss;
             kl += w * o.kl;
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(TB) void policy_tokens_k(Seqs q, const int* cnt, co
     begin();
     const Weights w(q, cnt, total, l);
     while (item < items) {
-        const float ws = w.of(q, cnt, item, a.per_seq, l.red);
+        const double ws = w.of(q, cnt, item, a.per_seq, l.red);
         for (; t < hi; t += TB) {
             const Token now = next;
             if (t + TB < hi) next = Token(q, a, t + TB);
@@ -250,15 +251,15 @@ __device__ __forceinline__ Totals small_totals(const Seqs& q, SmallSeqs& l, int6
     n.alive = block_total(n.alive, red);
     return n;
 }
-__device__ __forceinline__ float small_weight(const SmallSeqs& l, const Totals& n, int t, int per_seq) {
+__device__ __forceinline__ double small_weight(const SmallSeqs& l, const Totals& n, int t, int per_seq) {
     const int s = l.seq[t];
-    return s < 0 ? 0.f : (float)(per_seq ? 1.0 / ((double)n.alive * (double)l.cnt[s]) : 1.0 / (double)n.n);
+    return s < 0 ? 0.0 : per_seq ? 1.0 / ((double)n.alive * (double)l.cnt[s]) : 1.0 / (double)n.n;
 }
 __global__ __launch_bounds__(kSmallBlock) void weight_small_k(Seqs q, int per_seq, float* weight) {
     __shared__ SmallSeqs l;
     __shared__ int64_t red[kSmallBlock / kWave];
     const Totals n = small_totals(q, l, red);
-    for (int t = threadIdx.x; t < q.n; t += kSmallBlock) weight[t] = small_weight(l, n, t, per_seq);
+    for (int t = threadIdx.x; t < q.n; t += kSmallBlock) weight[t] = (float)small_weight(l, n, t, per_seq);
 }
 __global__ __launch_bounds__(kSmallBlock) void policy_small_k(Seqs q, PolicyTokens a, float* loss_out) {
     __shared__ SmallSeqs l;
