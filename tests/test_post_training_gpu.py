@@ -714,11 +714,13 @@ def test_two_streams_with_their_own_workspaces(env):
             assert torch.equal(x, t)
 
 
-def test_captured_and_replayed(env):
+# one block for the tokens, several launches, rows split over workgroups
+@pytest.mark.parametrize("n,V", [(96, 2050), (9000, 130), (60, 131079)])
+def test_captured_and_replayed(env, n, V):
     """A step's loss, gradient, preference loss and clipping in one graph, replayed on new inputs."""
     torch, ops = env
-    n, V, S = 96, 2050, 4
-    st = torch.tensor([0, 20, 50, 51, 90], device="cuda")
+    S = 4
+    st = torch.tensor([0, 20, 50, 51, n - 6], device="cuda")
     z, y, _ = make_logits(torch, n, V, torch.bfloat16, 1)
     old, ref, adv = (torch.empty(n, device="cuda") for _ in range(3))
     f = lambda *s: torch.empty(*s, device="cuda")  # noqa: E731
