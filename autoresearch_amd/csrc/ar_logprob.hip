@@ -595,7 +595,8 @@ void launch(hipStream_t st, const LpRows& a) {
 
 size_t lp_scratch(LpOp op, bool bf16_logits, int64_t n, int64_t V) {
     const int parts = n > 0 ? split_parts(op, n, V, bf16_logits ? Row<bf16>::E : Row<float>::E) : 1;
-    return parts > 1 ? n * (parts * sizeof(MaxSum) + (op == LpOp::POLICY ? sizeof(PolicyToken) : 0) + sizeof(float)) : 0;
+    const size_t token = op == LpOp::POLICY ? sizeof(PolicyToken) : 0;
+    return parts > 1 ? n * (parts * sizeof(MaxSum) + token + sizeof(float)) : 0;
 }
 
 int32_t lp_rows(hipStream_t st, LpOp op, bool bf16_logits, const LpRows& a, const char* nm) {
@@ -611,7 +612,7 @@ int32_t check_rows(const char* nm, const void* logits, int32_t logits_bf16, cons
     AR_CHECK_ARG(n >= 0 && V > 0, "%s: bad shape", nm);
     AR_CHECK_ARG(n == 0 || (logits && targets), "%s: null pointer", nm);
     AR_CHECK_ARG(logits_bf16 == 0 || logits_bf16 == 1, "%s: logits_bf16 must be 0 or 1", nm);
-    if (n > INT32_MAX || V > INT32_MAX / 2)
+    if (n > INT32_MAX || V > (int64_t(1) << 30))
         return set_error(AR_EUNSUPPORTED, "%s: more than 2^31 - 1 tokens or 2^30 logits per token", nm);
     const size_t es = logits_bf16 ? 2 : 4, bytes = (size_t)n * V * es;
     AR_CHECK_ARG(((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(grad)) & (es - 1)) == 0,

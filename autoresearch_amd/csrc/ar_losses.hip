@@ -509,7 +509,7 @@ int32_t check_seqs(const char* nm, const int64_t* targets, const int64_t* seq_st
     AR_CHECK_ARG(n >= 0 && S >= 0 && V > 0, "%s: bad shape", nm);
     AR_CHECK_ARG(n == 0 || targets, "%s: null pointer", nm);
     AR_CHECK_ARG(seq_start || S == 1, "%s: without seq_start the tokens are one sequence", nm);
-    if (n > INT32_MAX || S > INT32_MAX / 2)
+    if (n > INT32_MAX || S > (int64_t(1) << 30))
         return set_error(AR_EUNSUPPORTED, "%s: more than 2^31 - 1 tokens or 2^30 sequences", nm);
     return AR_OK;
 }
@@ -645,7 +645,8 @@ extern "C" int32_t ar_preference_loss(ar_stream_t stream, float* loss_out, float
                                       int64_t num_tokens, int64_t num_pairs, int64_t vocab_size, float loss_scale) {
     const char* nm = "preference_loss";
     AR_CHECK_ARG(loss_out && seq_start && (num_tokens <= 0 || logp), "%s: null pointer", nm);
-    AR_CHECK_ARG(num_pairs >= 0 && num_pairs <= INT32_MAX / 4, "%s: bad number of pairs", nm);
+    AR_CHECK_ARG(num_pairs >= 0, "%s: bad number of pairs", nm);
+    if (num_pairs > (1 << 29)) return set_error(AR_EUNSUPPORTED, "%s: more than 2^29 pairs", nm);
     if (const int32_t r = check_seqs(nm, targets, seq_start, num_tokens, 2 * num_pairs, vocab_size)) return r;
     AR_CHECK_ARG(beta == beta && label_smoothing >= 0.0 && label_smoothing <= 1.0,
                  "%s: label_smoothing must lie in [0, 1]", nm);

@@ -286,11 +286,13 @@ int32_t ar_muon_step(ar_stream_t stream, float* params, float* grads, float* mom
  * A token counts if 0 <= target < vocab_size and, where there are sequences,
  * it lies in one: sequence s holds tokens seq_start[s] .. seq_start[s + 1] - 1
  * (device, num_seqs + 1 ascending offsets in [0, num_tokens]; with others, which
- * tokens count is not defined, but nothing outside the arrays is touched).  A token that does not count has
- * log-probability 0 and gradient 0, whatever its logits or other inputs hold;
- * its logits are not read.  Sums over tokens are fp64, in a fixed order.
+ * tokens count is not defined, but nothing outside the arrays is touched).  A
+ * token that does not count has log-probability 0 and gradient 0, whatever its
+ * logits or other inputs hold; its logits are not read.  Sums over tokens are
+ * fp64, in a fixed order.
  *
- * num_tokens up to 2^31 - 1, vocab_size up to 2^30 (AR_EUNSUPPORTED above).
+ * num_tokens up to 2^31 - 1, vocab_size and num_seqs up to 2^30
+ * (AR_EUNSUPPORTED above).
  * Calls on up to 128 tokens with a vocabulary of 65536 or more take scratch
  * from the workspace.
  * Arrays of no elements may be NULL. */
@@ -313,8 +315,8 @@ int32_t ar_token_logprob_bwd(ar_stream_t stream, void* grad_logits, const void* 
  * Without a token that counts all outputs are 0.  old_logp NULL: old_logp =
  * logp, held fixed (r = 1).  ref_logp NULL: no KL term (kl_coef 0, loss_out[1]
  * 0).  grad_logp NULL: the loss alone; it may be logp or another input, not
- * overlap one in part.  seq_start NULL: the
- * tokens are one sequence (num_seqs 1).  May take scratch from the workspace. */
+ * overlap one in part.  seq_start NULL: the tokens are one sequence (num_seqs
+ * 1).  May take scratch from the workspace. */
 int32_t ar_policy_loss(ar_stream_t stream, float* loss_out, float* grad_logp, const float* logp,
                        const float* old_logp, const float* ref_logp, const float* advantages, const int64_t* targets,
                        const int64_t* seq_start, double clip_low, double clip_high, double kl_coef, int32_t per_seq,

@@ -133,6 +133,14 @@ def test_preference(lib, kw, word):
     refused(lib, preference(lib, **kw), EINVAL, word)
 
 
+def test_more_than_there_is_room_for(lib):
+    refused(lib, preference(lib, P=(1 << 29) + 1), EUNSUPPORTED, "2^29")
+    for call in (policy, policy_logits):
+        refused(lib, call(lib, S=(1 << 30) + 1), EUNSUPPORTED, "2^30")
+    for call in ROWS:
+        refused(lib, call(lib, V=(1 << 30) + 1), EUNSUPPORTED, "2^30")
+
+
 def clip(lib, ptrs, sizes, bf16=None, outs=None, max_norm=1.0, norm=A["loss"], n=None):
     n = len(ptrs) if n is None else n
     arr = lambda t, v: None if v is None else (t * len(v))(*v)  # noqa: E731
